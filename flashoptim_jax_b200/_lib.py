@@ -29,6 +29,7 @@ EXPORTS = (
     "fo_step", "fo_step_ex", "fo_quantize_momentum", "fo_dequantize_momentum", "fo_quantize_variance",
     "fo_dequantize_variance", "fo_split", "fo_reconstruct", "fo_split_many", "fo_reconstruct_many", "fo_selftest", "fo_selftest_static", "fo_version",
     "fo_status_string", "fo_last_error", "fo_sq_norm", "fo_sq_norm_mixed", "fo_mean_sq_norm", "fo_step_scalars", "fo_step_scalars_schedule",
+    "fo_dropout", "fo_embed", "fo_embed_grad", "fo_embed_grad_workspace",
 )
 FO_SQ_NORM_WORKSPACE_BYTES = 16384
 
@@ -82,6 +83,35 @@ class FoSplitLeaf(ctypes.Structure):
 
 class FoArray(ctypes.Structure):
     _fields_ = [("data", ctypes.c_void_p), ("n", ctypes.c_uint64)]
+
+
+class FoDropout(ctypes.Structure):
+    _fields_ = [("p", ctypes.c_double), ("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64), ("dev_offset", ctypes.c_void_p),
+                ("dev_offset_bits", ctypes.c_int32), ("reserved", ctypes.c_uint32)]
+
+
+class FoEmbed(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("table_dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32), ("ecc_bits", ctypes.c_int32), ("ids_bits", ctypes.c_int32),
+        ("reserved", ctypes.c_uint32),
+        ("table", ctypes.c_void_p), ("ecc", ctypes.c_void_p), ("ids", ctypes.c_void_p), ("out", ctypes.c_void_p),
+        ("n_tokens", ctypes.c_uint64), ("rows", ctypes.c_uint64), ("dim", ctypes.c_uint64),
+        ("row_stride", ctypes.c_uint64), ("ecc_stride", ctypes.c_uint64),
+        ("scale", ctypes.c_double), ("dropout", FoDropout),
+    ]
+
+
+class FoEmbedGrad(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("dy_dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32), ("ids_bits", ctypes.c_int32), ("accumulate", ctypes.c_int32),
+        ("reserved", ctypes.c_uint32),
+        ("dy", ctypes.c_void_p), ("ids", ctypes.c_void_p), ("out", ctypes.c_void_p),
+        ("n_tokens", ctypes.c_uint64), ("rows", ctypes.c_uint64), ("dim", ctypes.c_uint64), ("dy_stride", ctypes.c_uint64),
+        ("scale", ctypes.c_double), ("dropout", FoDropout),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64),
+    ]
 
 
 class NativeLibraryError(RuntimeError):
@@ -140,6 +170,14 @@ def lib() -> ctypes.CDLL:
     cdll.fo_step_scalars.argtypes = [vp, vp, ctypes.c_float, ctypes.c_float, ctypes.c_float, vp, vp, vp]
     cdll.fo_step_scalars_schedule.restype = ctypes.c_int
     cdll.fo_step_scalars_schedule.argtypes = [vp, i32, ctypes.POINTER(ctypes.c_float), ctypes.c_float, ctypes.c_float, vp, vp, vp]
+    cdll.fo_dropout.restype = ctypes.c_int
+    cdll.fo_dropout.argtypes = [vp, vp, vp, i32, u64, ctypes.POINTER(FoDropout), vp]
+    cdll.fo_embed.restype = ctypes.c_int
+    cdll.fo_embed.argtypes = [ctypes.POINTER(FoEmbed), vp]
+    cdll.fo_embed_grad.restype = ctypes.c_int
+    cdll.fo_embed_grad.argtypes = [ctypes.POINTER(FoEmbedGrad), vp]
+    cdll.fo_embed_grad_workspace.restype = ctypes.c_int
+    cdll.fo_embed_grad_workspace.argtypes = [u64, u64, u64, ctypes.POINTER(u64)]
     cdll.fo_version.restype = ctypes.c_int
     cdll.fo_version.argtypes = []
     cdll.fo_status_string.restype = ctypes.c_char_p

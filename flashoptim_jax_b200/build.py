@@ -62,7 +62,7 @@ def _has_kernel(oname: str, kname: str, mname: str) -> bool:
 
 def _units(shapes=None, ffi_dir: str | None = None) -> List[Tuple[str, str, List[str]]]:
     shapes = _SHAPES if shapes is None else shapes
-    units = [(name, name + ".cu", []) for name in ("fo_api", "fo_codec", "fo_selftest", "fo_norm")]
+    units = [(name, name + ".cu", []) for name in ("fo_api", "fo_codec", "fo_selftest", "fo_norm", "fo_dropout", "fo_embed", "fo_embed_grad")]
     if ffi_dir is not None:
         units.append(("fo_ffi", "fo_ffi.cc", ["-x", "cu", f"-I{ffi_dir}"]))
 

@@ -19,6 +19,7 @@ from . import _engine as eng
 from . import _lib
 from . import tree as pytree
 from ._dev import as_tensor
+from .embedding import dense_gradients
 from .utils import FlashOptimizer
 
 
@@ -37,7 +38,10 @@ def clip_by_global_norm(tx: FlashOptimizer, max_norm: float) -> FlashOptimizer:
         return {"clip": (), "opt": tx.init(params)}
 
     def step_fn(params: Any, state: Any, grads: Any):
-        sq = global_sq_norm(grads)
+        sq = _lib.host().sq_norm(grads)
+        if sq is None:
+            grads = dense_gradients(params, grads)
+            sq = global_sq_norm(grads)
         with eng.grad_clip(sq, max_norm):
             params, opt_state = tx.step(params, state["opt"], grads)
         return params, {"clip": (), "opt": opt_state}

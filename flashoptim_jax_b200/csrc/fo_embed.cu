@@ -1,0 +1,206 @@
+// Embedding lookup:  out[n, :] = drop(scale * W[ids[n], :]), W stored in fp32 or 16 bits, or split into a 16-bit
+// parameter and its error-correction code (the rows are then the fp32 weights that reconstruct_leaf gives).
+#include "fo_tokens.cuh"
+
+namespace fo {
+
+constexpr int kEmbedThreads = 256;
+
+struct EmbedParams {
+  const void* table;
+  const void* ecc;
+  const void* ids;
+  void* out;
+  unsigned long long n_tokens, rows, dim;
+  unsigned long long row_stride, ecc_stride;  // elements
+  int32_t ids_bits, out_f32;
+  float factor;  // scale, and 1 / (1 - p)
+  Drop drop;
+};
+
+template <int ECC>
+struct EccOct {
+  uint4 a;
+  FO_DEVI void load(const void* p) {
+    if constexpr (ECC == 16) a = *(const uint4*)p;
+    if constexpr (ECC == 8) { const uint2 b = *(const uint2*)p; a = make_uint4(b.x, b.y, 0u, 0u); }
+  }
+  FO_DEVI int get(const int j) const {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+    if constexpr (ECC == 16) return (int)(short)(w[j / 2] >> (16 * (j & 1)));
+    if constexpr (ECC == 8) return (int)(signed char)(w[j / 4] >> (8 * (j & 3)));
+    return 0;
+  }
+};
+
+template <int DT, int ECC>
+FO_DEVI float weight(const void* table, const void* ecc, const unsigned long long i, const unsigned long long i_ecc) {
+  if constexpr (ECC == 0) return load1<DT>(table, i);
+  else return fast::reconstruct<DT, ECC>(((const unsigned short*)table)[i], ECC == 16 ? (int)((const short*)ecc)[i_ecc] : (int)((const signed char*)ecc)[i_ecc]);
+}
+
+// A negative id is no token: zeros.  An id behind the last row reads nothing: a row of NaN, seen in the loss.
+FO_DEVI float without_row(const long long id) { return id < 0 ? 0.0f : __int_as_float(0x7FC00000); }
+
+// Eight elements of a row per thread, kOcts threads' widths apart: the ids, then the rows, then the results.  Bound by HBM.
+// dim is a multiple of 8, all rows start on 16 bytes (codes of 8 bits: on 8).  INDEX: 32 bits where dim / 8 * n_tokens fits them.
+template <int DT, int ECC, typename INDEX, int OCTS>
+__global__ void __launch_bounds__(kEmbedThreads) embed_kernel(const __grid_constant__ EmbedParams p) {
+  chain_wait();
+  chain_release();
+  Drop d = p.drop;
+  resolve_offset(d);
+  const INDEX per_row = (INDEX)(p.dim / 8), octs = (INDEX)p.n_tokens * per_row;
+  const INDEX q0 = (INDEX)blockIdx.x * (kEmbedThreads * OCTS) + threadIdx.x;
+  Oct<DT> x[OCTS];
+  EccOct<ECC> e[OCTS];
+  long long id[OCTS];
+  INDEX col[OCTS];
+#pragma unroll
+  for (int k = 0; k < OCTS; ++k) {
+    const INDEX q = q0 + k * kEmbedThreads;
+    if (q >= octs) break;
+    const INDEX n = q / per_row;
+    col[k] = q - n * per_row;
+    id[k] = id_at(p.ids, p.ids_bits, n);
+  }
+#pragma unroll
+  for (int k = 0; k < OCTS; ++k) {
+    const INDEX q = q0 + k * kEmbedThreads;
+    if (q >= octs) break;
+    if (id[k] < 0 || (unsigned long long)id[k] >= p.rows) continue;
+    x[k].load((const char*)p.table + ((unsigned long long)id[k] * p.row_stride + (unsigned long long)col[k] * 8) * size_of(DT));
+    if constexpr (ECC != 0) e[k].load((const char*)p.ecc + ((unsigned long long)id[k] * p.ecc_stride + (unsigned long long)col[k] * 8) * (ECC / 8));
+  }
+#pragma unroll
+  for (int k = 0; k < OCTS; ++k) {
+    const INDEX q = q0 + k * kEmbedThreads;
+    if (q >= octs) break;
+    const uint32_t keep = d.on ? keep8(d, q) : 0xFFu;
+    float v[8];
+    if (id[k] < 0 || (unsigned long long)id[k] >= p.rows) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = without_row(id[k]);
+    } else if constexpr (ECC == 0) {
+      x[k].get(v);
+    } else {
+      const uint32_t w[4] = {x[k].a.x, x[k].a.y, x[k].a.z, x[k].a.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = fast::reconstruct<DT, ECC>((w[j / 2] >> (16 * (j & 1))) & 0xFFFFu, e[k].get(j));
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (keep >> j & 1u) != 0 ? fmul(v[j], p.factor) : 0.0f;
+    if (DT == FO_F32 || p.out_f32) {
+      Oct<FO_F32> y;
+      y.set(v);
+      y.store((char*)p.out + (unsigned long long)q * 32);
+    } else {
+      Oct<DT> y;
+      y.set(v);
+      y.store((char*)p.out + (unsigned long long)q * 16);
+    }
+  }
+}
+
+// Any width, stride and alignment: eight neighbouring results per thread, which may lie in several rows.
+template <int DT, int ECC>
+__global__ void __launch_bounds__(kEmbedThreads) embed_any_kernel(const __grid_constant__ EmbedParams p) {
+  chain_wait();
+  chain_release();
+  Drop d = p.drop;
+  resolve_offset(d);
+  const unsigned long long total = p.n_tokens * p.dim, octs = (total + 7) / 8;
+  for (unsigned long long q = (unsigned long long)blockIdx.x * kEmbedThreads + threadIdx.x; q < octs; q += (unsigned long long)gridDim.x * kEmbedThreads) {
+    const uint32_t keep = d.on ? keep8(d, q) : 0xFFu;
+    unsigned long long n = q * 8 / p.dim, c = q * 8 - n * p.dim;
+    long long id = id_at(p.ids, p.ids_bits, n);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (q * 8 + j < total) {
+        if (c == p.dim) {
+          c = 0;
+          id = id_at(p.ids, p.ids_bits, ++n);
+        }
+        v[j] = id < 0 || (unsigned long long)id >= p.rows ? without_row(id) : weight<DT, ECC>(p.table, p.ecc, (unsigned long long)id * p.row_stride + c, (unsigned long long)id * p.ecc_stride + c);
+        ++c;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (keep >> j & 1u) != 0 ? fmul(v[j], p.factor) : 0.0f;
+    if (q * 8 + 8 <= total && on_16_bytes(p.out)) {
+      if (DT == FO_F32 || p.out_f32) {
+        Oct<FO_F32> y;
+        y.set(v);
+        y.store((char*)p.out + q * 32);
+      } else {
+        Oct<DT> y;
+        y.set(v);
+        y.store((char*)p.out + q * 16);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (q * 8 + j < total) {
+          if (DT == FO_F32 || p.out_f32) store1<FO_F32>(p.out, q * 8 + j, v[j]);
+          else store1<DT>(p.out, q * 8 + j, v[j]);
+        }
+    }
+  }
+}
+
+template <int DT, int ECC>
+static int launch_embed(const EmbedParams& p, const bool vectors, cudaStream_t stream) {
+  const unsigned long long octs = vectors ? p.n_tokens * (p.dim / 8) : (p.n_tokens * p.dim + 7) / 8;
+  bool chained = true;
+  cudaError_t e;
+  if (!vectors) {
+    const unsigned long long blocks = (octs + kEmbedThreads - 1) / kEmbedThreads;
+    e = launch_chained(embed_any_kernel<DT, ECC>, (unsigned int)(blocks < 0x7FFFFFFFull ? blocks : 0x7FFFFFFFull), (unsigned int)kEmbedThreads, 0, chained, stream, p);
+  } else {
+    constexpr int kOcts = 2;
+    const unsigned long long blocks = (octs + kEmbedThreads * kOcts - 1) / (kEmbedThreads * kOcts);
+    if (blocks > 0x7FFFFFFFull) return fail(FO_ERR_TOO_LARGE, "fo_embed: %llu tokens of %llu elements exceed one launch", p.n_tokens, p.dim);
+    void (*kernel)(const EmbedParams) = octs < 0xFFFF0000ull ? embed_kernel<DT, ECC, uint32_t, kOcts> : embed_kernel<DT, ECC, unsigned long long, kOcts>;
+    e = launch_chained(kernel, (unsigned int)blocks, (unsigned int)kEmbedThreads, 0, chained, stream, p);
+  }
+  return e == cudaSuccess ? FO_OK : fail(FO_ERR_CUDA, "fo_embed: launch failed: %s", cudaGetErrorString(e));
+}
+
+}  // namespace fo
+
+using namespace fo;
+
+extern "C" int fo_embed(const FoEmbed* f, void* stream) {
+  if (f == nullptr) return fail(FO_ERR_INVALID_ARG, "fo_embed: null descriptor");
+  if (f->struct_size != sizeof(FoEmbed)) return fail(FO_ERR_INVALID_ARG, "fo_embed: struct_size %u != %zu (ABI mismatch)", f->struct_size, sizeof(FoEmbed));
+  if (f->table_dtype < FO_F32 || f->table_dtype > FO_F16) return fail(FO_ERR_INVALID_ARG, "fo_embed: bad table_dtype %d", f->table_dtype);
+  if (f->out_dtype != FO_F32 && f->out_dtype != f->table_dtype) return fail(FO_ERR_INVALID_ARG, "fo_embed: out_dtype %d (the table's or fp32)", f->out_dtype);
+  if (f->ecc_bits != 0 && f->ecc_bits != 8 && f->ecc_bits != 16) return fail(FO_ERR_INVALID_ARG, "fo_embed: ecc_bits %d", f->ecc_bits);
+  if (f->ecc_bits != 0 && f->table_dtype == FO_F32) return fail(FO_ERR_INVALID_ARG, "fo_embed: an fp32 table carries no ECC");
+  if (f->ids_bits != 32 && f->ids_bits != 64) return fail(FO_ERR_INVALID_ARG, "fo_embed: ids_bits %d (32 or 64)", f->ids_bits);
+  EmbedParams p;
+  double factor;
+  if (!make_drop(&f->dropout, p.drop, factor)) return fail(FO_ERR_INVALID_ARG, "fo_embed: p = %g (it lies in [0, 1]), dev_offset_bits = %d (32 or 64)", f->dropout.p, f->dropout.dev_offset_bits);
+  if (f->n_tokens == 0 || f->dim == 0) return FO_OK;
+  if (f->ids == nullptr || f->out == nullptr || (f->rows > 0 && (f->table == nullptr || (f->ecc_bits != 0 && f->ecc == nullptr))))
+    return fail(FO_ERR_INVALID_ARG, "fo_embed: null pointer");
+  if (f->row_stride < f->dim || (f->ecc_bits != 0 && f->ecc_stride < f->dim)) return fail(FO_ERR_INVALID_ARG, "fo_embed: rows %llu elements apart are %llu long", (unsigned long long)f->row_stride, (unsigned long long)f->dim);
+  // element numbers, and byte addresses in the table, stay below 2^60
+  if (f->n_tokens >> 32 || f->dim >> 28 || f->rows >> 32 || f->row_stride >> 28 || f->ecc_stride >> 28)
+    return fail(FO_ERR_TOO_LARGE, "fo_embed: %llu tokens, %llu rows of %llu elements", (unsigned long long)f->n_tokens, (unsigned long long)f->rows, (unsigned long long)f->dim);
+  p.table = f->table; p.ecc = f->ecc; p.ids = f->ids; p.out = f->out;
+  p.n_tokens = f->n_tokens; p.rows = f->rows; p.dim = f->dim;
+  p.row_stride = f->row_stride; p.ecc_stride = f->ecc_stride;
+  p.ids_bits = f->ids_bits;
+  p.out_f32 = f->out_dtype == FO_F32;
+  p.factor = (float)((double)f->scale * factor);
+  const int size = size_of(f->table_dtype), code = f->ecc_bits / 8;
+  const bool vectors = f->dim % 8 == 0 && on_16_bytes(f->table) && f->row_stride * size % 16 == 0 && on_16_bytes(f->out) &&
+                       (code == 0 || ((uintptr_t)f->ecc % (8 * code) == 0 && f->ecc_stride % 8 == 0));
+#define X(D, E) \
+  if (f->table_dtype == D && f->ecc_bits == E) return launch_embed<D, E>(p, vectors, (cudaStream_t)stream);
+  X(FO_F32, 0) X(FO_BF16, 0) X(FO_BF16, 8) X(FO_BF16, 16) X(FO_F16, 0) X(FO_F16, 8) X(FO_F16, 16)
+#undef X
+  return fail(FO_ERR_INVALID_ARG, "fo_embed: table_dtype %d with ecc_bits %d", f->table_dtype, f->ecc_bits);
+}

@@ -37,6 +37,7 @@ from . import tree as pytree
 from . import utils
 from ._dev import DTYPE_CODE, as_tensor
 from .adamw import adam_hyper
+from .embedding import TokenGradient
 from .lion import lion_hyper
 from .sgd import sgd_hyper
 
@@ -567,12 +568,16 @@ class Zero1Optimizer:
             if treedef != self.treedef:
                 raise ValueError(f"{self.name} gradients must match parameter structure")
             for mine, theirs in zip(pytree.tree_leaves(self.grads), leaves):
-                theirs = as_tensor(theirs)
+                tokens = theirs if isinstance(theirs, TokenGradient) else None
+                theirs = as_tensor(theirs) if tokens is None else tokens.dy
                 if theirs.dtype != mine.dtype and theirs.element_size() > mine.element_size():
                     # the flat gradient buffers (and the reduce-scatter) have the parameters' dtype
                     raise TypeError(f"{self.name}: a {theirs.dtype} gradient would be narrowed to the {mine.dtype} gradient "
                                     "buffer of its leaf; cast it yourself or write into `.grads` directly")
-                mine.copy_(theirs.to(mine.dtype).reshape(mine.shape))
+                if tokens is not None:
+                    tokens.dense(mine, out=mine)
+                else:
+                    mine.copy_(theirs.to(mine.dtype).reshape(mine.shape))
         if self._pipelined():
             if not (do_rs and do_ag):
                 raise ValueError("the sliced pipeline runs whole steps only")

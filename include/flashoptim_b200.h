@@ -277,6 +277,65 @@ typedef struct FoSplitLeaf {
 int fo_split_many(const FoSplitLeaf* leaves, uint32_t n_leaves, int32_t param_dtype, int32_t ecc_bits, void* cuda_stream);
 int fo_reconstruct_many(const FoSplitLeaf* leaves, uint32_t n_leaves, int32_t param_dtype, int32_t ecc_bits, void* cuda_stream);
 
+/* ---- the token end of a training step ----------------------------------------------------------------------------
+ * No counterpart in the reference, which takes the gradients of a pytree as they come: what makes the gradient of its largest leaf, an
+ * embedding table, and the lookup and dropout that go with it.
+ *
+ * Dropout from a counter-based generator.  Element e (row-major) of a call stays where its uniform 32-bit number is at
+ * least round(p 2^32), and is then multiplied by 1 / (1 - p); otherwise it becomes 0 whatever it held.  The number is a function of
+ * (seed, offset, e): 16 bits from the block e / 8 of Philox4x32-10 under the key `seed` with the counter (e / 8, offset), and, where these
+ * equal the threshold's upper half, 16 more from the block with the counter's bit 63 set.  Nothing is stored: a backward pass gives the same
+ * three again.  *dev_offset (device, 32- or 64-bit signed as dev_offset_bits says; NULL: none) is added to the offset when the kernel runs, so that
+ * a captured call drops other elements at each replay. */
+typedef struct FoDropout {
+  double p; /* 0 ... 1 */
+  uint64_t seed, offset;
+  const void* dev_offset;
+  int32_t dev_offset_bits;
+  uint32_t reserved;
+} FoDropout;
+
+/* y = x * keep / (1 - p), plus residual where it is not NULL; n elements of one dtype.  y may be x or residual itself. */
+int fo_dropout(const void* x, const void* residual, void* y, int32_t dtype, uint64_t n, const FoDropout* dropout, void* cuda_stream);
+
+/* out[t, :] = drop(scale * W[ids[t], :]), W of `rows` rows of `dim` elements, row_stride apart.  With ecc_bits 8 or 16, W is what fo_reconstruct
+ * makes of (table, ecc), whose rows are ecc_stride apart.  out: n_tokens x dim without gaps, in the table's dtype or fp32; rounded once.  A negative id
+ * is no token: a row of zeros.  An id behind the last row reads nothing: a row of NaN. */
+typedef struct FoEmbed {
+  uint32_t struct_size;
+  int32_t table_dtype, out_dtype, ecc_bits, ids_bits;
+  uint32_t reserved;
+  const void* table;
+  const void* ecc;
+  const void* ids;
+  void* out;
+  uint64_t n_tokens, rows, dim, row_stride, ecc_stride;
+  double scale;
+  FoDropout dropout; /* p 0: none */
+} FoEmbed;
+int fo_embed(const FoEmbed* desc, void* cuda_stream);
+
+/* The gradient of fo_embed: out[v, :] = sum over the tokens t with ids[t] = v of drop'(scale * dy[t, :]), in fp32, in an order that depends on
+ * the ids alone (same inputs, same bits), rounded once; rows without a token are cleared.  accumulate != 0: the sum is added to
+ * out[v, :] in fp32 before that rounding, and rows without a token are left alone.  out: rows x dim without gaps; dy: n_tokens rows, dy_stride apart.
+ * Ids that name no row are left out.  workspace: fo_embed_grad_workspace bytes of device memory, aligned to 16, which calls on one stream
+ * may share.  Fewer than 2^31 - 1 tokens and rows, dim below 2^24. */
+typedef struct FoEmbedGrad {
+  uint32_t struct_size;
+  int32_t dy_dtype, out_dtype, ids_bits, accumulate;
+  uint32_t reserved;
+  const void* dy;
+  const void* ids;
+  void* out;
+  uint64_t n_tokens, rows, dim, dy_stride;
+  double scale;
+  FoDropout dropout; /* as the lookup's */
+  void* workspace;
+  uint64_t workspace_bytes;
+} FoEmbedGrad;
+int fo_embed_grad_workspace(uint64_t rows, uint64_t dim, uint64_t n_tokens, uint64_t* bytes);
+int fo_embed_grad(const FoEmbedGrad* desc, void* cuda_stream);
+
 /*
  * Device self-checks of the exact-arithmetic shortcuts the kernels use (no counterpart in
  * the reference).  Each runs a sweep on the current device and writes the number of inputs
