@@ -48,8 +48,8 @@ template <int DT, int ECC, typename INDEX, int OCTS>
 __global__ void __launch_bounds__(kEmbedThreads) embed_kernel(const __grid_constant__ EmbedParams p) {
   chain_wait();
   chain_release();
-  Drop d = p.drop;
-  resolve_offset(d);
+  const Drop& d = p.drop;
+  const uint2 off = drop_offset(d);
   const INDEX per_row = (INDEX)(p.dim / 8), octs = (INDEX)p.n_tokens * per_row;
   const INDEX q0 = (INDEX)blockIdx.x * (kEmbedThreads * OCTS) + threadIdx.x;
   Oct<DT> x[OCTS];
@@ -72,11 +72,15 @@ __global__ void __launch_bounds__(kEmbedThreads) embed_kernel(const __grid_const
     x[k].load((const char*)p.table + ((unsigned long long)id[k] * p.row_stride + (unsigned long long)col[k] * 8) * size_of(DT));
     if constexpr (ECC != 0) e[k].load((const char*)p.ecc + ((unsigned long long)id[k] * p.ecc_stride + (unsigned long long)col[k] * 8) * (ECC / 8));
   }
+  uint4 w[OCTS];  // drawn while the rows are on their way
+  if (d.on) {
+#pragma unroll
+    for (int k = 0; k < OCTS; ++k) w[k] = draw8(d, off, q0 + k * kEmbedThreads);
+  }
 #pragma unroll
   for (int k = 0; k < OCTS; ++k) {
     const INDEX q = q0 + k * kEmbedThreads;
     if (q >= octs) break;
-    const uint32_t keep = d.on ? keep8(d, q) : 0xFFu;
     float v[8];
     if (id[k] < 0 || (unsigned long long)id[k] >= p.rows) {
 #pragma unroll
@@ -84,12 +88,16 @@ __global__ void __launch_bounds__(kEmbedThreads) embed_kernel(const __grid_const
     } else if constexpr (ECC == 0) {
       x[k].get(v);
     } else {
-      const uint32_t w[4] = {x[k].a.x, x[k].a.y, x[k].a.z, x[k].a.w};
+      const uint32_t h[4] = {x[k].a.x, x[k].a.y, x[k].a.z, x[k].a.w};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = fast::reconstruct<DT, ECC>((w[j / 2] >> (16 * (j & 1))) & 0xFFFFu, e[k].get(j));
+      for (int j = 0; j < 8; ++j) v[j] = fast::reconstruct<DT, ECC>((h[j / 2] >> (16 * (j & 1))) & 0xFFFFu, e[k].get(j));
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = (keep >> j & 1u) != 0 ? fmul(v[j], p.factor) : 0.0f;
+    for (int j = 0; j < 8; ++j) v[j] = fmul(v[j], p.factor);
+    if (d.on) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = stays(d, w[k], j) ? v[j] : 0.0f;
+    }
     if (DT == FO_F32 || p.out_f32) {
       Oct<FO_F32> y;
       y.set(v);
@@ -102,68 +110,59 @@ __global__ void __launch_bounds__(kEmbedThreads) embed_kernel(const __grid_const
   }
 }
 
-// Any width, stride and alignment: eight neighbouring results per thread, which may lie in several rows.
+// Any width, stride and alignment: 256 neighbouring results per warp, which may lie in several rows, neighbours in neighbouring lanes; each lane draws
+// for eight neighbours and hands them on.
 template <int DT, int ECC>
 __global__ void __launch_bounds__(kEmbedThreads) embed_any_kernel(const __grid_constant__ EmbedParams p) {
   chain_wait();
   chain_release();
-  Drop d = p.drop;
-  resolve_offset(d);
-  const unsigned long long total = p.n_tokens * p.dim, octs = (total + 7) / 8;
-  for (unsigned long long q = (unsigned long long)blockIdx.x * kEmbedThreads + threadIdx.x; q < octs; q += (unsigned long long)gridDim.x * kEmbedThreads) {
-    const uint32_t keep = d.on ? keep8(d, q) : 0xFFu;
-    unsigned long long n = q * 8 / p.dim, c = q * 8 - n * p.dim;
-    long long id = id_at(p.ids, p.ids_bits, n);
-    float v[8];
+  const Drop& d = p.drop;
+  const uint2 off = drop_offset(d);
+  const int lane = threadIdx.x & 31;
+  const unsigned long long total = p.n_tokens * p.dim, first = ((unsigned long long)blockIdx.x * kEmbedThreads + (threadIdx.x & ~31u)) * 8;
+  unsigned long long n, c;
+  if (first + 256 < 0xFFFFFFFFull && p.dim <= 0xFFFFFFFFull) {
+    n = (uint32_t)(first + lane) / (uint32_t)p.dim;
+    c = (uint32_t)(first + lane) - (uint32_t)n * (uint32_t)p.dim;
+  } else {
+    n = (first + lane) / p.dim;
+    c = first + lane - n * p.dim;
+  }
+  long long id[8];
+  unsigned long long col[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (q * 8 + j < total) {
-        if (c == p.dim) {
-          c = 0;
-          id = id_at(p.ids, p.ids_bits, ++n);
-        }
-        v[j] = id < 0 || (unsigned long long)id >= p.rows ? without_row(id) : weight<DT, ECC>(p.table, p.ecc, (unsigned long long)id * p.row_stride + c, (unsigned long long)id * p.ecc_stride + c);
-        ++c;
-      }
-    }
+  for (int j = 0; j < 8; ++j) {
+    col[j] = c;
+    id[j] = first + j * 32 + lane < total ? id_at(p.ids, p.ids_bits, n) : -1;
+    for (c += 32; c >= p.dim; c -= p.dim) ++n;
+  }
+  float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = (keep >> j & 1u) != 0 ? fmul(v[j], p.factor) : 0.0f;
-    if (q * 8 + 8 <= total && on_16_bytes(p.out)) {
-      if (DT == FO_F32 || p.out_f32) {
-        Oct<FO_F32> y;
-        y.set(v);
-        y.store((char*)p.out + q * 32);
-      } else {
-        Oct<DT> y;
-        y.set(v);
-        y.store((char*)p.out + q * 16);
-      }
-    } else {
+  for (int j = 0; j < 8; ++j)
+    v[j] = id[j] < 0 || (unsigned long long)id[j] >= p.rows
+               ? without_row(id[j])
+               : weight<DT, ECC>(p.table, p.ecc, (unsigned long long)id[j] * p.row_stride + col[j], (unsigned long long)id[j] * p.ecc_stride + col[j]);
+  const uint32_t mine = d.on ? keep8(d, off, first / 8 + lane) : 0xFFu;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (q * 8 + j < total) {
-          if (DT == FO_F32 || p.out_f32) store1<FO_F32>(p.out, q * 8 + j, v[j]);
-          else store1<DT>(p.out, q * 8 + j, v[j]);
-        }
-    }
+  for (int j = 0; j < 8; ++j) {
+    const unsigned long long e = first + j * 32 + lane;
+    v[j] = (__shfl_sync(~0u, mine, j * 4 + lane / 8) >> (lane & 7) & 1u) != 0 ? fmul(v[j], p.factor) : 0.0f;
+    if (e >= total) continue;
+    if (DT == FO_F32 || p.out_f32) store1<FO_F32>(p.out, e, v[j]);
+    else store1<DT>(p.out, e, v[j]);
   }
 }
 
 template <int DT, int ECC>
 static int launch_embed(const EmbedParams& p, const bool vectors, cudaStream_t stream) {
+  constexpr int kOcts = 2;
   const unsigned long long octs = vectors ? p.n_tokens * (p.dim / 8) : (p.n_tokens * p.dim + 7) / 8;
+  const unsigned long long per_block = (unsigned long long)kEmbedThreads * (vectors ? kOcts : 1), blocks = (octs + per_block - 1) / per_block;
+  if (blocks > 0x7FFFFFFFull) return fail(FO_ERR_TOO_LARGE, "fo_embed: %llu tokens of %llu elements exceed one launch", p.n_tokens, p.dim);
+  void (*kernel)(const EmbedParams) = embed_any_kernel<DT, ECC>;
+  if (vectors) kernel = octs < 0xFFFF0000ull ? embed_kernel<DT, ECC, uint32_t, kOcts> : embed_kernel<DT, ECC, unsigned long long, kOcts>;
   bool chained = true;
-  cudaError_t e;
-  if (!vectors) {
-    const unsigned long long blocks = (octs + kEmbedThreads - 1) / kEmbedThreads;
-    e = launch_chained(embed_any_kernel<DT, ECC>, (unsigned int)(blocks < 0x7FFFFFFFull ? blocks : 0x7FFFFFFFull), (unsigned int)kEmbedThreads, 0, chained, stream, p);
-  } else {
-    constexpr int kOcts = 2;
-    const unsigned long long blocks = (octs + kEmbedThreads * kOcts - 1) / (kEmbedThreads * kOcts);
-    if (blocks > 0x7FFFFFFFull) return fail(FO_ERR_TOO_LARGE, "fo_embed: %llu tokens of %llu elements exceed one launch", p.n_tokens, p.dim);
-    void (*kernel)(const EmbedParams) = octs < 0xFFFF0000ull ? embed_kernel<DT, ECC, uint32_t, kOcts> : embed_kernel<DT, ECC, unsigned long long, kOcts>;
-    e = launch_chained(kernel, (unsigned int)blocks, (unsigned int)kEmbedThreads, 0, chained, stream, p);
-  }
+  const cudaError_t e = launch_chained(kernel, (unsigned int)blocks, (unsigned int)kEmbedThreads, 0, chained, stream, p);
   return e == cudaSuccess ? FO_OK : fail(FO_ERR_CUDA, "fo_embed: launch failed: %s", cudaGetErrorString(e));
 }
 

@@ -1,44 +1,43 @@
 // Gradient of an embedding lookup:  dW[v, :] (+)= sum over the tokens n with ids[n] = v, in ascending n, of
 // scale * keep / (1 - p) * dY[n, :], in fp32, rounded once.
 //
-// Three steps.  (1) The tokens are sorted by id, stably (so the order of every sum is fixed: same inputs, same bits, no atomics on
-// values).  (2) The sorted tokens are cut into chunks of equal length whatever their ids, so that an id that half of all
-// tokens carry costs no more than others: a warp adds up 256 columns of one chunk, writes the rows whose tokens lie all in the
-// chunk, and leaves a partial sum of the row at either end that does not.  (3) The partial sums of a row are added up.
-#include <cooperative_groups.h>
-
+// Two steps.  (1) The tokens are sorted by id, stably (so the order of every sum is fixed: same inputs, same bits, no atomics on
+// values), which also says where each row's tokens begin.  (2) The sorted tokens are cut into chunks of equal length whatever their ids, so that an id
+// that half of all tokens carry costs no more than others: a warp adds up 256 columns of one chunk and writes the rows whose tokens lie all in
+// the chunk; of the row at either end that does not, it leaves a partial sum, and the warp that leaves a row's last one adds
+// them up.  The blocks behind clear the rows without a token.
 #include "fo_tokens.cuh"
 
 namespace fo {
-
-namespace cg = cooperative_groups;
 
 constexpr int kSms = 148;
 
 // ---- sizes and the workspace ----------------------------------------------------------------------------------------
 constexpr int kTileCols = 256;     // columns of a warp: eight per lane
-constexpr int kSumThreads = 256;
-constexpr int kLeastChunk = 4;     // tokens
-constexpr int kSumWarps = kSms * 32;  // wanted
+constexpr int kSumThreads = 256, kSumBlocksPerSm = 3;
+constexpr int kLeastChunk = 8;     // tokens
+constexpr int kSumWarps = kSms * kSumBlocksPerSm * kSumThreads / 32;  // wanted: all of them resident at once
+
+// The sort by rows, in one launch or two: 128 blocks, a 16-bit counter per row and warp.
+constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
+constexpr int kSortRows = 2048;                      // of a block, at most
+constexpr uint32_t kSortBlocks = 128;
+constexpr unsigned long long kSortMost = 65536;      // tokens
+constexpr unsigned long long kSortAlone = 4096;  // of which up to so many take one launch
+// The sort over several launches: tiles of 4096 tokens, digits of at most nine bits.
+constexpr int kDigitMax = 9, kBinsMax = 1 << kDigitMax;
+constexpr int kRadixThreads = 512, kRadixRounds = 8, kRadixTile = kRadixThreads * kRadixRounds;
 
 struct GradPlan {
   bool several;  // the sort takes several launches
   uint32_t tiles, chunk, chunks;
   uint32_t blocks;  // of such a sort
-  unsigned long long key[2], pos[2], hist, total, partial, bytes;  // offsets in the workspace
+  unsigned long long key[2], pos[2], starts, counters, hist, total, partial, bytes;  // offsets in the workspace
 };
-
-constexpr int kDigitMax = 9, kBinsMax = 1 << kDigitMax;
-// The sort of one cluster: eight blocks, which hold all tokens in shared memory.
-constexpr int kCluster = 8, kSortThreads = 1024, kSortRounds = 8;
-constexpr unsigned long long kSortMost = (unsigned long long)kCluster * kSortThreads * kSortRounds;
-constexpr int kSortRowBits = 27;  // of the rows, of which a bit each lies in the shared memory of the blocks beside it
-// The sort over several launches: tiles of 4096 tokens.
-constexpr int kRadixThreads = 512, kRadixRounds = 8, kRadixTile = kRadixThreads * kRadixRounds;
 
 static GradPlan plan_of(const unsigned long long rows, const unsigned long long dim, const unsigned long long n) {
   GradPlan g = {};
-  g.several = n > kSortMost || rows >> kSortRowBits != 0;
+  g.several = n > kSortMost || rows >= (unsigned long long)kSortBlocks * kSortRows;
   g.tiles = (uint32_t)((dim + kTileCols - 1) / kTileCols);
   unsigned long long chunk = (n * g.tiles + kSumWarps - 1) / kSumWarps;
   if (chunk < kLeastChunk) chunk = kLeastChunk;
@@ -52,10 +51,14 @@ static GradPlan plan_of(const unsigned long long rows, const unsigned long long 
     at += (bytes + 255) / 256 * 256;
     return here;
   };
-  for (int i = 0; i < (g.several ? 2 : 1); ++i) {
-    g.key[i] = take(4 * n);
-    g.pos[i] = take(4 * n);
+  const unsigned long long dealt = (n + 2 * kSortThreads - 1) / (2 * kSortThreads) * (2 * kSortThreads);
+  for (int i = 0; i < (n > kSortAlone || g.several ? 2 : 1); ++i) {
+    g.key[i] = take(4 * dealt);
+    g.pos[i] = take(4 * dealt);
   }
+  g.starts = take(4 * (rows + 1));
+  g.counters = take(12ull * g.chunks * g.tiles);
+  if (!g.several && n > kSortAlone) g.hist = take(4ull * kSortBlocks * (kSortMost / (2 * kSortThreads)));
   if (g.several) {
     g.hist = take(4ull * kBinsMax * g.blocks);
     g.total = take(4ull * kBinsMax);
@@ -66,16 +69,6 @@ static GradPlan plan_of(const unsigned long long rows, const unsigned long long 
 }
 
 // ---- (1) the sort ----------------------------------------------------------------------------------------------------
-struct SortParams {
-  const void* ids;
-  uint32_t* key_out;
-  uint32_t* pos_out;
-  void* out;  // the gradient, whose rows without a token are cleared meanwhile; null: none are
-  unsigned long long row_bytes;
-  uint32_t n, rows, m;  // m: tokens of a block
-  int32_t ids_bits, passes, digit_bits;
-};
-
 // Ids that name no row sort behind all rows.
 FO_DEVI uint32_t key_of(const long long id, const uint32_t rows) { return id < 0 || id >= (long long)rows ? rows : (uint32_t)id; }
 
@@ -92,141 +85,284 @@ FO_DEVI void clear_bytes(char* a, char* const b, const int lane) {
   if (down + 2 * lane < b) *(unsigned short*)(down + 2 * lane) = 0;
 }
 
-// exclusive sum over the first kBinsMax threads of a block; all threads call it
-FO_DEVI uint32_t scan_bins(const uint32_t v, uint32_t* warp_sums) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// Exclusive sum over the threads of a block of at most 1024; all of them call it.
+FO_DEVI uint32_t scan_block(const uint32_t v, uint32_t* warp_sums, uint32_t& all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   uint32_t x = v;
 #pragma unroll
   for (int s = 1; s < 32; s <<= 1) {
     const uint32_t y = __shfl_up_sync(~0u, x, s);
     if (lane >= s) x += y;
   }
-  if (lane == 31 && warp < kBinsMax / 32) warp_sums[warp] = x;
+  if (lane == 31) warp_sums[warp] = x;
   __syncthreads();
-  uint32_t before = 0;
-  for (int w = 0; w < warp && w < kBinsMax / 32; ++w) before += warp_sums[w];
+  uint32_t sum = lane < warps ? warp_sums[lane] : 0u, before = lane < warp ? sum : 0u;
+  sum = __reduce_add_sync(~0u, sum);
+  before = __reduce_add_sync(~0u, before);
   __syncthreads();
+  all = sum;
   return before + x - v;
 }
 
 // The place of a lane's token among those of its warp with the same digit so far; `counts`: the warp's, one per digit.  The lanes of one digit
-// are found at once, the first of them counts for all.
-FO_DEVI uint32_t rank_in_warp(const uint32_t digit, const bool valid, unsigned short* counts, const int lane) {
-  const uint32_t same = __match_any_sync(~0u, valid ? digit : 0xFFFFFFFFu);
+// find one another bit by bit, where there are several digits among them; the first of them counts for all.
+FO_DEVI uint32_t rank_in_warp(const uint32_t digit, const bool valid, const int bits, unsigned short* counts, const int lane) {
+  uint32_t same = __ballot_sync(~0u, valid);
+  const uint32_t one_of_them = __shfl_sync(~0u, digit, __ffs(same) - 1);
+  if (__any_sync(~0u, valid && digit != one_of_them))
+#pragma unroll 1
+    for (int b = 0; b < bits; ++b) {
+      const bool one = (digit >> b & 1u) != 0;
+      const uint32_t ones = __ballot_sync(~0u, one);
+      same &= one ? ones : ~ones;
+    }
+  const uint32_t before = __popc(same & ((1u << lane) - 1u));
   uint32_t rank = 0;
-  if (valid) rank = counts[digit] + __popc(same & ((1u << lane) - 1u));
+  if (valid) rank = counts[digit] + before;
   __syncwarp();
-  if (valid && (same & ((1u << lane) - 1u)) == 0) counts[digit] += (unsigned short)__popc(same);
+  if (valid && before == 0) counts[digit] = (unsigned short)(rank + __popc(same));
   __syncwarp();
   return rank;
 }
 
-struct SortShared {
-  unsigned short counts[kSortThreads / 32][kBinsMax];
-  uint32_t hist[2][kBinsMax];
-  uint32_t base[kBinsMax];
-  uint32_t warp_sums[kBinsMax / 32];
+struct SortParams {
+  const void* ids;
+  uint32_t* key_out;
+  uint32_t* pos_out;
+  uint32_t* starts;  // [rows + 1]: where the tokens of each row begin, in the order of slot_of
+  uint32_t* counters;
+  uint32_t n, rows, n_counters;
+  int32_t ids_bits, row_bits;  // of a row's number within a block
 };
 
-// Up to kSortMost tokens: one cluster sorts them, least digit first, its blocks' shared memory holding all keys and positions
-// (a pass moves them through the cluster's shared memory, not through the L2, and its barriers are the hardware's), while the other
-// blocks clear the rows of the gradient that no token names.
-__global__ void __launch_bounds__(kSortThreads) __cluster_dims__(kCluster, 1, 1) sort_kernel(const __grid_constant__ SortParams p) {
+// The order in which the one-launch sort puts the rows: those of a block behind one another, block after block, row r belonging to block r % kSortBlocks.
+// (Frequent ids are neighbours in most vocabularies: of text, the first 1 / 148 of GPT-2's rows has half of all tokens.)
+__host__ __device__ inline uint32_t rows_before(const uint32_t block, const uint32_t rows) { return block * (rows / kSortBlocks) + min(block, rows % kSortBlocks); }
+FO_DEVI uint32_t slot_of(const uint32_t row, const uint32_t rows) { return rows_before(row % kSortBlocks, rows) + row / kSortBlocks; }
+
+// Up to kSortMost tokens, in one launch and without a word between its blocks: each block has 1 / 128 of the rows.  It reads all ids (from the L2: at 64
+// bytes a clock 16384 of them take 1 us), counts those of blocks in front of it, which is where its tokens begin in the order, and
+// those of each of its rows, warp by warp, each warp having the tokens behind those of the one before; then it walks over the ids again and puts its
+// tokens in their places.  Eight blocks that sorted by digits through the shared memory of a cluster took 12.4 us for 8192 tokens, mostly waiting
+// for one another.  Loops stay loops: unrolled, their code took longer to fetch than to run.
+__global__ void __launch_bounds__(kSortThreads) sort_kernel(const __grid_constant__ SortParams p) {
   chain_wait();
   chain_release();
   extern __shared__ __align__(16) unsigned char sort_mem[];
+  __shared__ uint32_t warp_sums[kSortWarps];
+  unsigned short* const counts = (unsigned short*)sort_mem;  // [warp][row]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (blockIdx.x >= kCluster) {
-    // this block's rows, a bit for each that a token names
-    uint32_t* const named = (uint32_t*)sort_mem;
-    const uint32_t f = blockIdx.x - kCluster, fs = gridDim.x - kCluster;
-    const uint32_t first = (uint32_t)((unsigned long long)p.rows * f / fs), last = (uint32_t)((unsigned long long)p.rows * (f + 1) / fs);
-    for (uint32_t i = threadIdx.x; i < (last - first + 31) / 32; i += kSortThreads) named[i] = 0;
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < p.n; i += kSortThreads) {
-      const uint32_t k = key_of(id_at(p.ids, p.ids_bits, i), p.rows);
-      if (k >= first && k < last) atomicOr(&named[(k - first) / 32], 1u << ((k - first) & 31));
-    }
-    __syncthreads();
-    for (uint32_t r = first + warp; r < last; r += kSortThreads / 32)
-      if ((named[(r - first) / 32] >> ((r - first) & 31) & 1u) == 0) {
-        char* const row = (char*)p.out + (unsigned long long)r * p.row_bytes;
-        clear_bytes(row, row + p.row_bytes, lane);
+  const uint32_t me = blockIdx.x, slots = rows_before(me, p.rows), mine = rows_before(me + 1, p.rows) - slots;
+  const uint32_t width = (p.rows / kSortBlocks + 2) & ~1u;  // of a warp's counters
+  uint32_t* const first = (uint32_t*)(sort_mem + (size_t)kSortWarps * width * 2);  // [row]
+  for (uint32_t i = threadIdx.x; i < kSortWarps * width / 2; i += kSortThreads) ((uint32_t*)counts)[i] = 0;
+  for (uint32_t i = me * kSortThreads + threadIdx.x; i < p.n_counters; i += gridDim.x * kSortThreads) p.counters[i] = 0;
+  const uint32_t rounds = (p.n + kSortThreads - 1) / kSortThreads;
+  const uint32_t i0 = warp * rounds * 32 + lane;
+  constexpr int kAtOnce = 4;
+  uint32_t below = 0;
+  __syncthreads();
+  // f(key, rank among the warp's tokens of its row, token) for this block's tokens
+  auto walk = [&](auto f) {
+#pragma unroll 1
+    for (uint32_t r0 = 0; r0 < rounds; r0 += kAtOnce) {
+      uint32_t key[kAtOnce];
+#pragma unroll
+      for (int r = 0; r < kAtOnce; ++r) {
+        const uint32_t i = i0 + (r0 + r) * 32;
+        key[r] = r0 + r < rounds && i < p.n ? key_of(id_at(p.ids, p.ids_bits, i), p.rows) : p.rows;
       }
-    return;
-  }
-  SortShared& s = *(SortShared*)sort_mem;
-  uint2* const buffer[2] = {(uint2*)(sort_mem + sizeof(SortShared)), (uint2*)(sort_mem + sizeof(SortShared)) + p.m};
-  cg::cluster_group cluster = cg::this_cluster();
-  const uint32_t me = blockIdx.x, begin = me * p.m;
-  const uint32_t mine = begin < p.n ? min(p.m, p.n - begin) : 0u;
-  const uint32_t rounds = (p.m + kSortThreads - 1) / kSortThreads;
-  const uint32_t at0 = warp * rounds * 32 + lane;  // a warp's tokens are neighbours, in rounds of 32
-  const uint32_t bins = 1u << p.digit_bits;
-  for (int pass = 0; pass < p.passes; ++pass) {
-    const int shift = pass * p.digit_bits;
-    for (uint32_t i = threadIdx.x; i < sizeof(s.counts) / 4; i += kSortThreads) ((uint32_t*)s.counts)[i] = 0;
-    __syncthreads();
-    uint2 item[kSortRounds];
-    uint32_t rank[kSortRounds];
 #pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) {
-      if (r >= (int)rounds) break;
-      const uint32_t i = at0 + r * 32;
-      const bool valid = i < mine;
-      if (valid) item[r] = pass == 0 ? make_uint2(key_of(id_at(p.ids, p.ids_bits, begin + i), p.rows), begin + i) : buffer[(pass - 1) & 1][i];
+      for (int r = 0; r < kAtOnce; ++r) {
+        const uint32_t block = key[r] % kSortBlocks;
+        const bool in = key[r] < p.rows && block == me;
+        below += key[r] < p.rows && block < me ? 1u : 0u;
+        if (!__any_sync(~0u, in)) continue;
+        const uint32_t rank = rank_in_warp(key[r] / kSortBlocks, in, p.row_bits, counts + warp * width, lane);
+        if (in) f(key[r], rank, i0 + (r0 + r) * 32);
+      }
     }
+  };
+  walk([](uint32_t, uint32_t, uint32_t) {});
+  uint32_t before, all;
+  scan_block(below, warp_sums, before);
+  // Per row: the warps' counts to places within the row, and its tokens; two rows a thread, neighbours.
+  uint32_t total[2] = {0u, 0u};
 #pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) {
-      if (r >= (int)rounds) break;
-      rank[r] = rank_in_warp((item[r].x >> shift) & (bins - 1), at0 + r * 32 < mine, s.counts[warp], lane);
-    }
-    __syncthreads();
-    if (threadIdx.x < kBinsMax) {  // digit by digit: the warps' counts to places, and the block's count
-      uint32_t sum = 0;
+  for (int j = 0; j < 2; ++j) {
+    const uint32_t row = threadIdx.x * 2 + j;
+    if (row < mine) {
 #pragma unroll 8
-      for (int w = 0; w < kSortThreads / 32; ++w) {
-        const uint32_t c = s.counts[w][threadIdx.x];
-        s.counts[w][threadIdx.x] = (unsigned short)sum;
-        sum += c;
-      }
-      s.hist[pass & 1][threadIdx.x] = sum;
-    }
-    cluster.sync();
-    uint32_t all = 0, before = 0;
-    if (threadIdx.x < kBinsMax) {
-      uint32_t h[kCluster];
-#pragma unroll
-      for (int b = 0; b < kCluster; ++b) h[b] = *cluster.map_shared_rank(&s.hist[pass & 1][threadIdx.x], b);
-#pragma unroll
-      for (int b = 0; b < kCluster; ++b) {
-        if (b < (int)me) before += h[b];
-        all += h[b];
+      for (int w = 0; w < kSortWarps; ++w) {
+        const uint32_t c = counts[w * width + row];
+        counts[w * width + row] = (unsigned short)total[j];
+        total[j] += c;
       }
     }
-    const uint32_t smaller = scan_bins(all, s.warp_sums);
-    if (threadIdx.x < kBinsMax) s.base[threadIdx.x] = smaller + before;
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) {
-      if (r >= (int)rounds) break;
-      if (at0 + r * 32 < mine) {
-        const uint32_t digit = (item[r].x >> shift) & (bins - 1);
-        const uint32_t to = s.base[digit] + s.counts[warp][digit] + rank[r];
-        if (pass + 1 == p.passes) {
-          p.key_out[to] = item[r].x;
-          p.pos_out[to] = item[r].y;
-        } else {
-          const uint32_t b = to / p.m;
-          cluster.map_shared_rank(buffer[pass & 1], b)[to - b * p.m] = item[r];
-        }
-      }
-    }
-    cluster.sync();  // also: no block ends while another reads its histogram
   }
+  const uint32_t at = before + scan_block(total[0] + total[1], warp_sums, all);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const uint32_t row = threadIdx.x * 2 + j;
+    if (row < mine) p.starts[slots + row] = first[row] = j == 0 ? at : at + total[0];
+  }
+  if (me == kSortBlocks - 1 && threadIdx.x == 0) p.starts[p.rows] = before + all;
+  __syncthreads();
+  // the counters now say where the warp's tokens begin: counting on gives each its place
+  walk([&](const uint32_t key, const uint32_t rank, const uint32_t i) {
+    const uint32_t to = first[key / kSortBlocks] + rank;
+    if (to >= p.n) return;  // (ids that another stream changed between the walks)
+    p.key_out[to] = key;
+    p.pos_out[to] = i;
+  });
 }
 
-// Clears the whole gradient; beside the first launch of a long sort.
+// More tokens than kSortAlone: two launches.  In the first, each block deals its 2048 tokens out to 128 piles by id % 128, each pile in the order of the
+// tokens; in the second, block b takes the b-th piles of all, block after block, and puts their tokens in the order of the rows.  The work does not grow
+// with blocks x tokens as above: 32768 tokens took 29 us there.
+constexpr int kDealTokens = 2 * kSortThreads;
+constexpr uint32_t kDealBlocksMost = kSortMost / kDealTokens;
+struct DealParams {
+  const void* ids;
+  uint32_t* pile_key;  // [block][kDealTokens]
+  uint32_t* pile_pos;
+  uint32_t* pile_size;  // [block][kSortBlocks]
+  uint32_t* key_out;
+  uint32_t* pos_out;
+  uint32_t* starts;
+  uint32_t* counters;
+  uint32_t n, rows, blocks, n_counters;
+  int32_t ids_bits, row_bits;
+};
+__global__ void __launch_bounds__(kSortThreads) deal_kernel(const __grid_constant__ DealParams p) {
+  chain_wait();
+  chain_release();
+  __shared__ unsigned short counts[kSortWarps][kSortBlocks];
+  __shared__ uint32_t warp_sums[kSortWarps], first[kSortBlocks];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t key[2], rank[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const uint32_t i = blockIdx.x * kDealTokens + warp * 64 + r * 32 + lane;
+    key[r] = i < p.n ? key_of(id_at(p.ids, p.ids_bits, i), p.rows) : p.rows;
+  }
+  for (uint32_t i = threadIdx.x; i < kSortWarps * kSortBlocks / 2; i += kSortThreads) ((uint32_t*)counts)[i] = 0;
+  for (uint32_t i = blockIdx.x * kSortThreads + threadIdx.x; i < p.n_counters; i += gridDim.x * kSortThreads) p.counters[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < 2; ++r) rank[r] = rank_in_warp(key[r] % kSortBlocks, key[r] < p.rows, 7, counts[warp], lane);
+  __syncthreads();
+  uint32_t size = 0, all;
+  if (threadIdx.x < kSortBlocks) {
+#pragma unroll 8
+    for (int w = 0; w < kSortWarps; ++w) {
+      const uint32_t c = counts[w][threadIdx.x];
+      counts[w][threadIdx.x] = (unsigned short)size;
+      size += c;
+    }
+    p.pile_size[blockIdx.x * kSortBlocks + threadIdx.x] = size;
+  }
+  const uint32_t at = scan_block(size, warp_sums, all);
+  if (threadIdx.x < kSortBlocks) first[threadIdx.x] = at;
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+    if (key[r] < p.rows) {
+      const uint32_t pile = key[r] % kSortBlocks, to = blockIdx.x * kDealTokens + first[pile] + counts[warp][pile] + rank[r];
+      p.pile_key[to] = key[r];
+      p.pile_pos[to] = blockIdx.x * kDealTokens + warp * 64 + r * 32 + lane;
+    }
+}
+__global__ void __launch_bounds__(kSortThreads) order_kernel(const __grid_constant__ DealParams p) {
+  chain_wait();
+  chain_release();
+  extern __shared__ __align__(16) unsigned char sort_mem[];
+  __shared__ uint32_t warp_sums[kSortWarps], pile_at[kDealBlocksMost], pile_begin[kDealBlocksMost + 1], smaller;
+  unsigned short* const counts = (unsigned short*)sort_mem;  // [warp][row]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t me = blockIdx.x, slots = rows_before(me, p.rows), mine = rows_before(me + 1, p.rows) - slots;
+  const uint32_t width = (p.rows / kSortBlocks + 2) & ~1u;
+  uint32_t* const first = (uint32_t*)(sort_mem + (size_t)kSortWarps * width * 2);  // [row]
+  // Where each block's pile begins and how large it is: a warp per block that dealt.
+  static_assert(kDealBlocksMost <= kSortWarps && kSortBlocks == 128, "a warp per block, four piles a lane");
+  if (warp < (int)p.blocks) {
+    const uint4 c = ((const uint4*)(p.pile_size + warp * kSortBlocks))[lane];
+    uint32_t before = 0;
+    before += lane * 4 < me ? c.x : 0u;
+    before += lane * 4 + 1 < me ? c.y : 0u;
+    before += lane * 4 + 2 < me ? c.z : 0u;
+    before += lane * 4 + 3 < me ? c.w : 0u;
+    before = __reduce_add_sync(~0u, before);
+    if (lane == (int)(me / 4)) {
+      pile_at[warp] = warp * kDealTokens + before;
+      pile_begin[warp + 1] = me % 4 == 0 ? c.x : (me % 4 == 1 ? c.y : (me % 4 == 2 ? c.z : c.w));
+    }
+    if (lane == 0) warp_sums[warp] = before;
+  }
+  for (uint32_t i = threadIdx.x; i < kSortWarps * width / 2; i += kSortThreads) ((uint32_t*)counts)[i] = 0;
+  __syncthreads();
+  if (warp == 0) {
+    uint32_t x = lane < (int)p.blocks ? pile_begin[lane + 1] : 0u;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const uint32_t y = __shfl_up_sync(~0u, x, s);
+      if (lane >= s) x += y;
+    }
+    if (lane < (int)kDealBlocksMost) pile_begin[lane + 1] = x;
+    if (lane == 0) pile_begin[0] = 0;
+    const uint32_t sum = __reduce_add_sync(~0u, lane < (int)p.blocks ? warp_sums[lane] : 0u);
+    if (lane == 0) smaller = sum;
+  }
+  __syncthreads();
+  const uint32_t tokens = pile_begin[p.blocks], before = smaller;
+  const uint32_t rounds = (tokens + kSortThreads - 1) / kSortThreads, warps = rounds == 0 ? 0u : (tokens + rounds * 32 - 1) / (rounds * 32);
+  unsigned short* const my_counts = counts + warp * width;
+  auto walk = [&](auto f) {
+    if (warp >= (int)warps) return;
+#pragma unroll 1
+    for (uint32_t r = 0; r < rounds; ++r) {
+      const uint32_t t = (warp * rounds + r) * 32 + lane;
+      uint32_t pile = 0;
+      for (uint32_t step = kDealBlocksMost / 2; step != 0; step /= 2)
+        if (pile + step < p.blocks && pile_begin[pile + step] <= t) pile += step;
+      const bool in = t < tokens;
+      const uint32_t from = pile_at[pile] + t - pile_begin[pile];
+      const uint32_t key = in ? p.pile_key[from] : 0u;
+      const uint32_t rank = rank_in_warp(key / kSortBlocks, in, p.row_bits, my_counts, lane);
+      if (in) f(key, rank, from);
+    }
+  };
+  walk([](uint32_t, uint32_t, uint32_t) {});
+  __syncthreads();
+  uint32_t total[2] = {0u, 0u}, all;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const uint32_t row = threadIdx.x * 2 + j;
+    if (row < mine) {
+#pragma unroll 4
+      for (uint32_t w = 0; w < warps; ++w) {
+        const uint32_t c = counts[w * width + row];
+        counts[w * width + row] = (unsigned short)total[j];
+        total[j] += c;
+      }
+    }
+  }
+  const uint32_t at = before + scan_block(total[0] + total[1], warp_sums, all);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const uint32_t row = threadIdx.x * 2 + j;
+    if (row < mine) p.starts[slots + row] = first[row] = j == 0 ? at : at + total[0];
+  }
+  if (me == kSortBlocks - 1 && threadIdx.x == 0) p.starts[p.rows] = before + all;
+  __syncthreads();
+  walk([&](const uint32_t key, const uint32_t rank, const uint32_t from) {
+    const uint32_t to = first[key / kSortBlocks] + rank;
+    p.key_out[to] = key;
+    p.pos_out[to] = p.pile_pos[from];
+  });
+}
+
+// More tokens, or more rows: least digit first, three launches per digit.
 struct RadixParams {
   const void* ids;
   const uint32_t* key_in;  // null: the ids
@@ -235,8 +371,6 @@ struct RadixParams {
   uint32_t* pos_out;
   uint32_t* hist;   // [bin][block]
   uint32_t* total;  // [bin]
-  void* out;
-  unsigned long long out_bytes;
   uint32_t n, rows, blocks;
   int32_t ids_bits, shift, digit_bits;
 };
@@ -245,13 +379,6 @@ FO_DEVI uint32_t radix_key(const RadixParams& p, const uint32_t i) { return p.ke
 __global__ void __launch_bounds__(kRadixThreads) radix_count_kernel(const __grid_constant__ RadixParams p) {
   chain_wait();
   chain_release();
-  if (blockIdx.x >= p.blocks) {
-    const unsigned long long warps = (unsigned long long)(gridDim.x - p.blocks) * (kRadixThreads / 32), w = (unsigned long long)(blockIdx.x - p.blocks) * (kRadixThreads / 32) + threadIdx.x / 32;
-    const unsigned long long step = 8192, pieces = (p.out_bytes + step - 1) / step;
-    for (unsigned long long i = w; i < pieces; i += warps)
-      clear_bytes((char*)p.out + i * step, (char*)p.out + (i + 1 < pieces ? (i + 1) * step : p.out_bytes), threadIdx.x & 31);
-    return;
-  }
   __shared__ uint32_t count[kBinsMax];
   for (int i = threadIdx.x; i < kBinsMax; i += kRadixThreads) count[i] = 0;
   __syncthreads();
@@ -299,7 +426,7 @@ __global__ void __launch_bounds__(kRadixThreads) radix_scatter_kernel(const __gr
   chain_release();
   __shared__ unsigned short counts[kRadixThreads / 32][kBinsMax];
   __shared__ uint32_t base[kBinsMax];
-  __shared__ uint32_t warp_sums[kBinsMax / 32];
+  __shared__ uint32_t warp_sums[kRadixThreads / 32];
   static_assert(kRadixThreads == kBinsMax, "a thread per digit");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (uint32_t i = threadIdx.x; i < sizeof(counts) / 4; i += kRadixThreads) ((uint32_t*)counts)[i] = 0;
@@ -310,7 +437,7 @@ __global__ void __launch_bounds__(kRadixThreads) radix_scatter_kernel(const __gr
 #pragma unroll
   for (int r = 0; r < kRadixRounds; ++r) key[r] = i0 + r * 32 < p.n ? radix_key(p, (uint32_t)(i0 + r * 32)) : 0u;
 #pragma unroll
-  for (int r = 0; r < kRadixRounds; ++r) rank[r] = rank_in_warp((key[r] >> p.shift) & mask, i0 + r * 32 < p.n, counts[warp], lane);
+  for (int r = 0; r < kRadixRounds; ++r) rank[r] = rank_in_warp((key[r] >> p.shift) & mask, i0 + r * 32 < p.n, p.digit_bits, counts[warp], lane);
   __syncthreads();
   uint32_t sum = 0;
 #pragma unroll 4
@@ -319,7 +446,8 @@ __global__ void __launch_bounds__(kRadixThreads) radix_scatter_kernel(const __gr
     counts[w][threadIdx.x] = (unsigned short)sum;
     sum += c;
   }
-  const uint32_t smaller = scan_bins(threadIdx.x <= mask ? p.total[threadIdx.x] : 0u, warp_sums);
+  uint32_t all;
+  const uint32_t smaller = scan_block(threadIdx.x <= mask ? p.total[threadIdx.x] : 0u, warp_sums, all);
   base[threadIdx.x] = smaller + p.hist[(unsigned long long)threadIdx.x * p.blocks + blockIdx.x];
   __syncthreads();
 #pragma unroll
@@ -333,166 +461,308 @@ __global__ void __launch_bounds__(kRadixThreads) radix_scatter_kernel(const __gr
   }
 }
 
-// ---- (2) and (3) the sums --------------------------------------------------------------------------------------------
+// Where the tokens of each row begin in the sorted order: a search per row.
+constexpr int kStartsThreads = 256;
+__global__ void __launch_bounds__(kStartsThreads) starts_kernel(const uint32_t* key, const uint32_t n, const uint32_t rows, uint32_t* starts, uint32_t* counters, const uint32_t n_counters) {
+  chain_wait();
+  chain_release();
+  const uint32_t i = blockIdx.x * kStartsThreads + threadIdx.x;
+  for (uint32_t c = i; c < n_counters; c += gridDim.x * kStartsThreads) counters[c] = 0;
+  if (i > rows) return;
+  uint32_t lo = 0, hi = n;  // the first token whose key is at least i
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    if (key[mid] < i) lo = mid + 1; else hi = mid;
+  }
+  starts[i] = lo;
+}
+
+// ---- (2) the sums ----------------------------------------------------------------------------------------------------
 struct SumParams {
   const void* dy;
   const uint32_t* key;
   const uint32_t* pos;
+  const uint32_t* starts;
+  uint32_t* counters;  // [3][chunk][tile]
   void* out;
-  float* partial;  // [chunk][first, last][tiles * kTileCols]
-  unsigned long long n, dim, dy_stride;
-  uint32_t rows, tiles, chunk, chunks;
-  int32_t out_dtype, accumulate, out_vectors;
+  float* partial;  // [chunk][first, last row][tiles * kTileCols]
+  unsigned long long dim;
+  unsigned long long row_bytes;  // of the gradient
+  uint32_t dy_bytes;             // between rows of dY
+  uint32_t rows, last_token, tiles, chunk, chunks;
+  int32_t dealt;  // starts is in the order of slot_of, not of the rows
   float factor;
   Drop drop;
 };
 
-// Eight columns of a row of the gradient, from c on (`count` of them inside the row).
-FO_DEVI void write_row(const SumParams& p, const uint32_t row, const unsigned long long c, const int count, float (&v)[8]) {
-  const unsigned long long at = (unsigned long long)row * p.dim + c;
-  auto go = [&](auto tag) {
-    constexpr int DT = decltype(tag)::value;
-    if (count == 8 && p.out_vectors) {
-      char* const to = (char*)p.out + at * size_of(DT);
-      Oct<DT> o;
-      if (p.accumulate) {
-        float old[8];
-        o.load(to);
-        o.get(old);
+// A lane's eight columns of a row of the gradient, `to` being where they begin: neighbours, or every 32nd, so that neighbours lie in neighbouring
+// lanes (`count`: columns from the lane's first one to the end of the tile).
+template <int OT, bool VECTORS>
+FO_DEVI void write_row(char* to, const int count, const float (&v)[8]) {
+  if constexpr (VECTORS) {
+    Oct<OT> o;
+    o.set(v);
+    if (count > 0) o.store(to);
+  } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = fadd(old[j], v[j]);
+    for (int j = 0; j < 8; ++j)
+      if (j * 32 < count) store1<OT>(to, j * 32, v[j]);
+  }
+}
+
+FO_DEVI void put8(float* to, const float (&v)[8]) {
+  __stcg((float4*)to, make_float4(v[0], v[1], v[2], v[3]));
+  __stcg((float4*)to + 1, make_float4(v[4], v[5], v[6], v[7]));
+}
+// true for all lanes of the warp that comes last of `of`
+FO_DEVI bool comes_last(uint32_t* counter, const uint32_t of, const int lane) {
+  __threadfence();
+  __syncwarp();
+  uint32_t seen = 0;
+  if (lane == 0) seen = atomicAdd(counter, 1u);
+  const bool last = __shfl_sync(~0u, seen, 0) + 1 == of;
+  if (last) __threadfence();
+  return last;
+}
+
+// Where the partial sum of a chunk's first row (begun in an earlier chunk) or last row (going on in the next) lies.
+FO_DEVI float* piece_at(const SumParams& p, const uint32_t chunk, const bool last, const uint32_t tile, const int lane) {
+  return p.partial + (((unsigned long long)chunk * 2 + (last ? 1 : 0)) * p.tiles + tile) * kTileCols + lane * 8;
+}
+// `chunk` has left its piece of a row whose tokens lie in the chunks c0 ... c1; true: it is the last to come, and the row's sum is in `sum`.  The pieces are
+// added up in groups of about the square root of their number, the groups by the last of them to come, in the order of the tokens whoever comes
+// last: the sum does not depend on it.  (One warp adding up 500 pieces would take longer than everything else.)
+FO_DEVI bool join_pieces(const SumParams& p, const uint32_t chunk, const uint32_t c0, const uint32_t c1, const uint32_t tile, const int lane, float (&sum)[8]) {
+  const uint32_t pieces = c1 - c0 + 1, group = max(16u, (uint32_t)ceilf(sqrtf((float)pieces)));
+  const uint32_t g = (chunk - c0) / group, groups = (pieces + group - 1) / group, cells = p.chunks * p.tiles;
+  // (a chunk may hold the first piece of one row and begin a group of another: they count apart)
+  uint32_t* counter = p.counters + (g == 0 ? 0u : cells) + (c0 + g * group) * p.tiles + tile;
+  uint32_t from = g * group, end = min(from + group, pieces), step = 1;
+#pragma unroll 1
+  for (int level = 0;; ++level) {
+    if (!comes_last(counter, (end - from + step - 1) / step, lane)) return false;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+      for (uint32_t i = from; i < end; i += 4 * step) {
+        float4 a[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (i + u * step < end) a[u] = __ldcg((const float4*)piece_at(p, c0 + i + u * step, i + u * step == 0, tile, lane) + h);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (i + u * step < end) t = make_float4(fadd(t.x, a[u].x), fadd(t.y, a[u].y), fadd(t.z, a[u].z), fadd(t.w, a[u].w));
       }
-      o.set(v);
-      o.store(to);
-    } else {
+      sum[4 * h] = t.x; sum[4 * h + 1] = t.y; sum[4 * h + 2] = t.z; sum[4 * h + 3] = t.w;
+    }
+    if (level == 1 || groups == 1) return true;
+    put8(piece_at(p, c0 + g * group, g == 0, tile, lane), sum);
+    counter = p.counters + 2 * cells + c0 * p.tiles + tile;
+    from = 0; end = pieces; step = group;
+  }
+}
+
+// A tile of a row of DT elements in shared memory.  VECTORS: eight neighbouring elements per lane, which copies and reads its own; otherwise every 32nd, and
+// 16-bit elements come as the words that hold them, with a half in front where the row starts in the middle of a word.
+template <int DT, bool VECTORS>
+struct Tile {
+  static constexpr int kBytes = kTileCols * size_of(DT) + (VECTORS || DT == FO_F32 ? 0 : 16);
+  // `from`: where the tile's first column lies; `count`: columns from the lane's first one on; edge: nothing in front of the tile or behind it may be touched
+  static FO_DEVI void fetch(unsigned char* stage, const char* from, const int columns, const int lane, const bool edge) {
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(stage);
+    if constexpr (VECTORS) {
+      if (lane * 8 < columns) {
+        copy_async16(to + lane * 16, from + lane * 8 * size_of(DT));
+        if constexpr (DT == FO_F32) copy_async16(to + 512 + lane * 16, from + lane * 32 + 16);
+      }
+    } else if constexpr (DT == FO_F32) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (j < count) store1<DT>(p.out, at + j, p.accumulate ? fadd(load1<DT>(p.out, at + j), v[j]) : v[j]);
+        if (j * 32 + lane < columns) copy_async4(to + (j * 32 + lane) * 4, from + (j * 32 + lane) * 4);
+    } else {
+      const int odd = (int)((uintptr_t)from >> 1) & 1;
+      if (edge) {
+        for (int e = lane; e < columns; e += 32) ((unsigned short*)stage)[odd + e] = ((const unsigned short*)from)[e];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 5; ++j)
+          if ((j < 4 || lane == 0) && 2 * (j * 32 + lane) - odd < columns) copy_async4(to + (j * 32 + lane) * 4, from - 2 * odd + (j * 32 + lane) * 4);
+      }
     }
-  };
-  if (p.out_dtype == FO_F32) go(std::integral_constant<int, FO_F32>{});
-  else if (p.out_dtype == FO_BF16) go(std::integral_constant<int, FO_BF16>{});
-  else go(std::integral_constant<int, FO_F16>{});
-}
+  }
+  static FO_DEVI void get(const unsigned char* stage, const char* from, const int lane, float (&v)[8]) {
+    if constexpr (VECTORS) {
+      Oct<DT> x;
+      x.a = *(const uint4*)(stage + lane * 16);
+      if constexpr (DT == FO_F32) x.b = *(const uint4*)(stage + 512 + lane * 16);
+      x.get(v);
+    } else {
+      const int odd = DT == FO_F32 ? 0 : (int)((uintptr_t)from >> 1) & 1;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = load1<DT>(stage, odd + j * 32 + lane);
+    }
+  }
+};
 
-// Bound by HBM: every row of dY is read once, in pieces of 512 bytes (1 KB in fp32) wherever the sort has put it; kAhead of them are in flight per warp.
-constexpr int kAhead = 4;
-template <int DT, bool VECTORS>
-__global__ void __launch_bounds__(kSumThreads) sum_kernel(const __grid_constant__ SumParams p) {
+// Bound by HBM: every row of dY is read once, in pieces of 512 bytes (1 KB in fp32) wherever the sort has put it.  A warp copies the pieces of the
+// next tokens into a ring in shared memory while it adds those at hand; where the gradient is added to, also what lies in the rows that begin among
+// them, which the sums start from.
+template <int DT, int OT, bool VECTORS, bool ACC>
+struct Ring {
+  static constexpr int kStages = DT == FO_F32 || ACC ? 4 : 8;
+  static constexpr int kOld = Tile<DT, VECTORS>::kBytes, kStage = kOld + (ACC ? Tile<OT, VECTORS>::kBytes : 0);
+  static constexpr int kWarp = kStages * kStage, kBlock = kWarp * (kSumThreads / 32);
+};
+template <int DT, int OT, bool VECTORS, bool DROP, bool ACC>
+__global__ void __launch_bounds__(kSumThreads, kSumBlocksPerSm) sum_kernel(const __grid_constant__ SumParams p) {
   chain_wait();
   chain_release();
-  Drop d = p.drop;
-  resolve_offset(d);
-  const int lane = threadIdx.x & 31;
-  const unsigned long long task = (unsigned long long)blockIdx.x * (kSumThreads / 32) + threadIdx.x / 32;
-  if (task >= (unsigned long long)p.chunks * p.tiles) return;
+  using R = Ring<DT, OT, VECTORS, ACC>;
+  constexpr int kStages = R::kStages;
+  extern __shared__ __align__(16) unsigned char rings[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+  const unsigned long long task = (unsigned long long)blockIdx.x * (kSumThreads / 32) + warp;
   const uint32_t tile = (uint32_t)(task % p.tiles), chunk = (uint32_t)(task / p.tiles);
-  const unsigned long long first = (unsigned long long)chunk * p.chunk, last = min(first + p.chunk, p.n);
-  const unsigned long long c = (unsigned long long)tile * kTileCols + lane * 8;
-  const int count = c >= p.dim ? 0 : (p.dim - c < 8 ? (int)(p.dim - c) : 8);
-  const uint32_t behind = last < p.n ? p.key[last] : 0xFFFFFFFFu;
-  uint32_t row = p.key[first];
-  bool open = first > 0 && p.key[first - 1] == row;  // the row began in an earlier chunk
-  float sum[8] = {};
-  float* const partial = p.partial + ((unsigned long long)chunk * 2 * p.tiles + tile) * kTileCols + lane * 8;
-  auto leave = [&](float* to) {
-    ((float4*)to)[0] = make_float4(sum[0], sum[1], sum[2], sum[3]);
-    ((float4*)to)[1] = make_float4(sum[4], sum[5], sum[6], sum[7]);
+  if (chunk >= p.chunks) return;
+  const uint32_t first = (uint32_t)((unsigned long long)chunk * p.chunk);
+  // keys and places of 32 tokens, one per lane; what lies behind the last token that names a row is nothing
+  const uint32_t n = p.starts[p.rows];
+  uint32_t key = first + lane <= p.last_token ? p.key[first + lane] : 0u, pos = first + lane <= p.last_token ? p.pos[first + lane] : 0u;
+  if (first >= n) return;
+  const uint32_t end = (uint32_t)min((unsigned long long)first + p.chunk, (unsigned long long)n);
+  const uint32_t last_row = p.key[end - 1];
+  const unsigned long long c0 = (unsigned long long)tile * kTileCols;
+  const int columns = p.dim - c0 < kTileCols ? (int)(p.dim - c0) : kTileCols;  // of this tile
+  const int count = columns - (VECTORS ? lane * 8 : lane);
+  const char* const from = (const char*)p.dy + c0 * size_of(DT);
+  char* const out = (char*)p.out + c0 * size_of(OT);
+  constexpr int kLaneOut = (VECTORS ? 8 : 1) * size_of(OT);
+  unsigned char* const ring = rings + warp * R::kWarp;
+  uint32_t row = __shfl_sync(~0u, key, 0);
+  const uint32_t first_row = row;
+  const uint32_t slot = p.dealt ? slot_of(row, p.rows) : row, row_begins = p.starts[slot], row_ends = p.starts[slot + 1];
+  const uint32_t last_ends = p.starts[(p.dealt ? slot_of(last_row, p.rows) : last_row) + 1];
+  const uint2 off = DROP ? drop_offset(p.drop) : make_uint2(0u, 0u);
+  bool opened = row_begins < first;  // in an earlier chunk
+  auto heads_of = [&](const uint32_t keys, const uint32_t before) {  // bit k: a row begins with token k of the 32
+    const uint32_t left = __shfl_up_sync(~0u, keys, 1);
+    return __ballot_sync(~0u, keys != (lane == 0 ? before : left));
   };
-  for (unsigned long long i0 = first; i0 < last && row < p.rows; i0 += kAhead) {
-    Oct<DT> x[kAhead];
-    float one[VECTORS ? 1 : kAhead][8];
-    uint32_t key[kAhead], pos[kAhead];
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      key[k] = i0 + k < last ? p.key[i0 + k] : 0xFFFFFFFFu;
-      pos[k] = i0 + k < last ? p.pos[i0 + k] : 0u;
+  uint32_t heads = heads_of(key, opened ? row : ~0u), next_key = 0, next_pos = 0, next_heads = 0;
+  // token `t` of the 64 at hand into a stage
+  auto fetch = [&](const uint32_t t, const uint32_t at, const int stage) {
+    unsigned char* const to = ring + stage * R::kStage;
+    Tile<DT, VECTORS>::fetch(to, from + (unsigned long long)at * p.dy_bytes, columns, lane, at == 0 || at == p.last_token);
+    if constexpr (ACC) {
+      const uint32_t r = __shfl_sync(~0u, t < 32 ? key : next_key, t & 31);
+      if (((t < 32 ? heads : next_heads) >> (t & 31) & 1u) != 0)
+        Tile<OT, VECTORS>::fetch(to + R::kOld, out + r * p.row_bytes, columns, lane, r == 0 || r == p.rows - 1);
     }
+  };
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      if (key[k] >= p.rows) break;
-      const unsigned long long at = (unsigned long long)pos[k] * p.dy_stride + c;
-      if constexpr (VECTORS) {
-        if (count > 0) x[k].load((const char*)p.dy + at * size_of(DT));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) one[k][j] = j < count ? load1<DT>(p.dy, at + j) : 0.0f;
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      if (i0 + k >= last) break;
-      if (key[k] != row) {  // (the same for the whole warp)
-        if (open) leave(partial);
-        else if (count > 0) write_row(p, row, c, count, sum);
-        open = false;
-        row = key[k];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum[j] = 0.0f;
-      }
-      if (row >= p.rows) break;
-      float v[8];
-      if constexpr (VECTORS) {
-        if (count > 0) x[k].get(v);
-        else
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = one[k][j];
-      }
-      const uint32_t keep = d.on ? keep8_from(d, (unsigned long long)pos[k] * p.dim + c) : 0xFFu;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sum[j] = fadd(sum[j], (keep >> j & 1u) != 0 ? fmul(v[j], p.factor) : 0.0f);
-    }
+  for (int k = 0; k < kStages - 1; ++k) {
+    const uint32_t at = __shfl_sync(~0u, pos, k);
+    if (first + k < end) fetch(k, at, k);
+    copy_commit();
   }
-  if (row >= p.rows) return;
-  if (open) leave(partial);  // (a row that began before and goes on behind leaves this one alone)
-  else if (behind == row) leave(partial + (unsigned long long)p.tiles * kTileCols);
-  else if (count > 0) write_row(p, row, c, count, sum);
+  float sum[8] = {};
+  bool any = false;  // a row began in this chunk
+#pragma unroll 1
+  for (uint32_t here = first; here < end; here += 32) {
+    next_key = here + 32 + lane < end ? p.key[here + 32 + lane] : 0u;
+    next_pos = here + 32 + lane < end ? p.pos[here + 32 + lane] : 0u;
+#pragma unroll 1
+    for (uint32_t k0 = 0; k0 < 32; k0 += kStages) {
+      if (k0 == 32 - kStages) next_heads = heads_of(next_key, __shfl_sync(~0u, key, 31));
+#pragma unroll
+      for (int s = 0; s < kStages; ++s) {
+        const uint32_t k = k0 + s, a = k + kStages - 1;
+        if (here + k >= end) break;
+        copy_wait<kStages - 2>();
+        if constexpr (!VECTORS) __syncwarp();  // the other lanes' copies are there, and the stage that is filled next has been read
+        const uint32_t ahead = __shfl_sync(~0u, a < 32 ? pos : next_pos, a & 31);
+        if (here + a < end) fetch(a, ahead, (s + kStages - 1) % kStages);
+        copy_commit();
+        const uint32_t at = DROP || !VECTORS ? __shfl_sync(~0u, pos, k) : 0u;
+        const unsigned long long e0 = at * p.dim + c0;
+        uint4 w = {};
+        if constexpr (DROP && VECTORS) w = draw8(p.drop, off, (e0 >> 3) + lane);
+        const unsigned char* const stage = ring + s * R::kStage;
+        if ((heads >> k & 1u) != 0) {  // (the same for the whole warp)
+          if (opened) put8(piece_at(p, chunk, false, tile, lane), sum);
+          else if (any) write_row<OT, VECTORS>(out + row * p.row_bytes + lane * kLaneOut, count, sum);
+          any = true;
+          opened = false;
+          row = __shfl_sync(~0u, key, k);
+          if constexpr (ACC) {
+            Tile<OT, VECTORS>::get(stage + R::kOld, out + row * p.row_bytes, lane, sum);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[j] = 0.0f;
+          }
+        }
+        float v[8];
+        Tile<DT, VECTORS>::get(stage, from + (unsigned long long)at * p.dy_bytes, lane, v);
+        if constexpr (DROP && VECTORS) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = stays(p.drop, w, j) ? v[j] : 0.0f;
+        } else if constexpr (DROP) {  // the warp's 256 columns lie in 32 or 33 blocks of eight
+          const uint32_t skew = (uint32_t)e0 & 7u;
+          const uint32_t low = keep8(p.drop, off, (e0 >> 3) + lane), high = skew != 0 ? keep8(p.drop, off, (e0 >> 3) + 32) : 0u;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t e = skew + j * 32 + lane;
+            const uint32_t bits = __shfl_sync(~0u, low, (e >> 3) & 31);
+            v[j] = ((e >= 256 ? high : bits) >> (e & 7) & 1u) != 0 ? v[j] : 0.0f;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[j] = __fmaf_rn(v[j], p.factor, sum[j]);
+      }
+      if (here + k0 + kStages >= end) break;
+    }
+    key = next_key;
+    pos = next_pos;
+    heads = next_heads;
+  }
+  const bool goes_on = last_ends > end;
+  if (opened) put8(piece_at(p, chunk, false, tile, lane), sum);
+  else if (goes_on) put8(piece_at(p, chunk, true, tile, lane), sum);
+  else write_row<OT, VECTORS>(out + row * p.row_bytes + lane * kLaneOut, count, sum);
+  // the pieces: of the row that began earlier, then of the one that goes on
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    if (which == 0 ? row_begins >= first : opened || !goes_on) continue;
+    const uint32_t c0 = which == 0 ? row_begins / p.chunk : chunk, c1 = ((which == 0 ? row_ends : last_ends) - 1) / p.chunk;
+    if (join_pieces(p, chunk, c0, c1, tile, lane, sum)) write_row<OT, VECTORS>(out + (which == 0 ? first_row : last_row) * p.row_bytes + lane * kLaneOut, count, sum);
+  }
 }
 
-// The rows whose tokens lie in several chunks: a block per chunk that such a row begins in, and tile of columns; the partial sums are
-// dealt out to the block's warps and added up in a fixed order.
-__global__ void __launch_bounds__(kSumThreads) join_kernel(const __grid_constant__ SumParams p) {
-  chain_wait();
+// Clears the rows without a token, in blocks in the order of the rows: 7.2 TB/s, where a block per SM that walks over its share of them gets 6.2 (128256
+// rows of 8 KB).  Its blocks start beside those of the sums, which are all resident by then, so that one's waiting hides behind the other's writing.
+constexpr int kClearThreads = 256, kClearBytes = 32768;  // of a block, about
+struct ClearParams {
+  const uint32_t* starts;
+  char* out;
+  unsigned long long row_bytes;
+  uint32_t rows, per_block;
+  int32_t dealt;  // starts is in the order of slot_of, not of the rows
+  int32_t wait;   // for the launch in front; otherwise that one has waited for the sort
+};
+__global__ void __launch_bounds__(kClearThreads) clear_kernel(const __grid_constant__ ClearParams p) {
+  if (p.wait) chain_wait();
   chain_release();
-  constexpr int kWarps = kSumThreads / 32;
-  __shared__ float part[kWarps][kTileCols];
-  const uint32_t tile = blockIdx.x % p.tiles, chunk = blockIdx.x / p.tiles;
-  const unsigned long long first = (unsigned long long)chunk * p.chunk, next = first + p.chunk;
-  if (next >= p.n) return;
-  const uint32_t row = p.key[next];
-  if (row >= p.rows || p.key[next - 1] != row) return;            // no row goes on from this chunk
-  if (p.key[first] == row && first > 0 && p.key[first - 1] == row) return;  // it began earlier
-  // the first chunk behind it that does not begin with the row
-  uint32_t lo = chunk + 1, hi = p.chunks;  // lo begins with it
-  while (hi - lo > 1) {
-    const uint32_t mid = lo + (hi - lo) / 2;
-    if (p.key[(unsigned long long)mid * p.chunk] == row) lo = mid; else hi = mid;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+  const uint32_t r0 = blockIdx.x * p.per_block, r1 = min(r0 + p.per_block, p.rows);
+  for (uint32_t r = r0 + warp; r < r1; r += kClearThreads / 32) {
+    const uint32_t s = p.dealt ? slot_of(r, p.rows) : r;
+    if (p.starts[s] == p.starts[s + 1]) {
+      char* const row = p.out + r * p.row_bytes;
+      clear_bytes(row, row + p.row_bytes, lane);
+    }
   }
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const unsigned long long width = (unsigned long long)p.tiles * kTileCols;
-  const float* const at = p.partial + (unsigned long long)tile * kTileCols + lane * 8;
-  float sum[8] = {};
-  auto add = [&](const float* from) {
-    const float4 a = ((const float4*)from)[0], b = ((const float4*)from)[1];
-    sum[0] = fadd(sum[0], a.x); sum[1] = fadd(sum[1], a.y); sum[2] = fadd(sum[2], a.z); sum[3] = fadd(sum[3], a.w);
-    sum[4] = fadd(sum[4], b.x); sum[5] = fadd(sum[5], b.y); sum[6] = fadd(sum[6], b.z); sum[7] = fadd(sum[7], b.w);
-  };
-  if (warp == 0) add(at + ((unsigned long long)chunk * 2 + 1) * width);
-#pragma unroll 4
-  for (uint32_t k = chunk + 1 + warp; k <= lo; k += kWarps) add(at + (unsigned long long)k * 2 * width);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) part[warp][lane * 8 + j] = sum[j];
-  __syncthreads();
-  if (warp != 0) return;
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    for (int w = 1; w < kWarps; ++w) sum[j] = fadd(sum[j], part[w][lane * 8 + j]);
-  const unsigned long long c = (unsigned long long)tile * kTileCols + lane * 8;
-  const int count = c >= p.dim ? 0 : (p.dim - c < 8 ? (int)(p.dim - c) : 8);
-  if (count > 0) write_row(p, row, c, count, sum);
+  chain_end();
 }
 
 static int sizes_ok(const char* who, uint64_t rows, uint64_t dim, uint64_t n) {
@@ -509,37 +779,40 @@ static void digits(uint32_t rows, int& passes, int& bits) {
   bits = (width + passes - 1) / passes;
 }
 
-constexpr int kSortSmem = 200 * 1024;
-static_assert(sizeof(SortShared) + 2 * sizeof(uint2) * kSortThreads * kSortRounds <= kSortSmem && (1u << kSortRowBits) / ((kSms - kCluster) / kCluster * kCluster) / 8 + 64 <= kSortSmem, "shared memory of the sort");
-static int sort_in_cluster(const FoEmbedGrad& f, const GradPlan& g, cudaStream_t stream) {
-  SortParams p = {};
+static int sort_by_rows(const FoEmbedGrad& f, const GradPlan& g, cudaStream_t stream) {
   char* const ws = (char*)f.workspace;
-  p.ids = f.ids; p.ids_bits = f.ids_bits;
-  p.key_out = (uint32_t*)(ws + g.key[0]); p.pos_out = (uint32_t*)(ws + g.pos[0]);
-  p.n = (uint32_t)f.n_tokens; p.rows = (uint32_t)f.rows;
-  p.m = (p.n + kCluster - 1) / kCluster;
-  digits(p.rows, p.passes, p.digit_bits);
-  p.out = f.accumulate ? nullptr : f.out;
-  p.row_bytes = f.dim * size_of(f.out_dtype);
-  unsigned int grid = kCluster;
-  if (!f.accumulate) grid += (kSms - kCluster) / kCluster * kCluster;
-  const size_t bits_bytes = (p.rows / (grid > kCluster ? grid - kCluster : 1) + 64) / 32 * 4;
-  size_t smem = sizeof(SortShared) + 2 * sizeof(uint2) * (size_t)p.m;
-  if (!f.accumulate && bits_bytes > smem) smem = bits_bytes;
+  const uint32_t n = (uint32_t)f.n_tokens, rows = (uint32_t)f.rows, n_counters = 3 * g.chunks * g.tiles;
+  uint32_t *const key = (uint32_t*)(ws + g.key[0]), *const pos = (uint32_t*)(ws + g.pos[0]), *const starts = (uint32_t*)(ws + g.starts), *const counters = (uint32_t*)(ws + g.counters);
+  int row_bits = 0;
+  while (rows / kSortBlocks >> row_bits != 0) ++row_bits;
+  const size_t width = (rows / kSortBlocks + 2) & ~1u, smem = kSortWarps * width * 2 + 4 * width;
+  constexpr int kMost = (kSortWarps * 2 + 4) * (kSortRows + 2);
+  static_assert(kMost <= 200 * 1024 && kSortRows == 2 * kSortThreads, "shared memory of the sort, and two rows a thread");
+  static_assert(kSortMost <= 65536, "places fit the counters");
   static std::atomic<uint64_t> ready{0};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return fail(FO_ERR_CUDA, "fo_embed_grad: cannot query the current device");
   if (dev >= 64 || (ready.load() >> dev & 1) == 0) {
-    if (cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortSmem) != cudaSuccess)
+    if (cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost) != cudaSuccess ||
+        cudaFuncSetAttribute(order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost) != cudaSuccess)
       return fail(FO_ERR_CUDA, "fo_embed_grad: cannot set the shared memory size");
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
   bool chained = true;
-  const cudaError_t e = launch_chained(sort_kernel, grid, (unsigned int)kSortThreads, (int)smem, chained, stream, p);
+  cudaError_t e;
+  if (n <= kSortAlone) {
+    const SortParams p = {f.ids, key, pos, starts, counters, n, rows, n_counters, f.ids_bits, row_bits};
+    e = launch_chained(sort_kernel, kSortBlocks, (unsigned int)kSortThreads, (int)smem, chained, stream, p);
+  } else {
+    const DealParams p = {f.ids, (uint32_t*)(ws + g.key[1]), (uint32_t*)(ws + g.pos[1]), (uint32_t*)(ws + g.hist), key, pos, starts, counters, n, rows,
+                          (n + kDealTokens - 1) / kDealTokens, n_counters, f.ids_bits, row_bits};
+    e = launch_chained(deal_kernel, p.blocks, (unsigned int)kSortThreads, 0, chained, stream, p);
+    if (e == cudaSuccess) e = launch_chained(order_kernel, kSortBlocks, (unsigned int)kSortThreads, (int)smem, chained, stream, p);
+  }
   return e == cudaSuccess ? FO_OK : fail(FO_ERR_CUDA, "fo_embed_grad: launch failed: %s", cudaGetErrorString(e));
 }
 
-// The sort over several launches; key[passes & 1] holds the result.
+// The sort over several launches; key[result] and pos[result] hold what comes of it.
 static int sort_in_memory(const FoEmbedGrad& f, const GradPlan& g, cudaStream_t stream, int& result) {
   char* const ws = (char*)f.workspace;
   RadixParams p = {};
@@ -548,7 +821,6 @@ static int sort_in_memory(const FoEmbedGrad& f, const GradPlan& g, cudaStream_t 
   p.ids = f.ids; p.ids_bits = f.ids_bits;
   p.hist = (uint32_t*)(ws + g.hist); p.total = (uint32_t*)(ws + g.total);
   p.n = (uint32_t)f.n_tokens; p.rows = (uint32_t)f.rows; p.blocks = g.blocks;
-  p.out = f.out; p.out_bytes = f.rows * f.dim * size_of(f.out_dtype);
   cudaError_t e = cudaSuccess;
   for (int pass = 0; pass < passes && e == cudaSuccess; ++pass) {
     p.key_in = pass == 0 ? nullptr : (const uint32_t*)(ws + g.key[(pass - 1) & 1]);
@@ -557,11 +829,14 @@ static int sort_in_memory(const FoEmbedGrad& f, const GradPlan& g, cudaStream_t 
     p.shift = pass * p.digit_bits;
     result = pass & 1;
     bool chained = true;
-    const unsigned int clearing = pass == 0 && !f.accumulate ? 2 * kSms : 0;
-    e = launch_chained(radix_count_kernel, p.blocks + clearing, (unsigned int)kRadixThreads, 0, chained, stream, p);
+    e = launch_chained(radix_count_kernel, p.blocks, (unsigned int)kRadixThreads, 0, chained, stream, p);
     if (e == cudaSuccess) e = launch_chained(radix_scan_kernel, 1u << p.digit_bits, (unsigned int)kRadixScanThreads, 0, chained, stream, p);
     if (e == cudaSuccess) e = launch_chained(radix_scatter_kernel, p.blocks, (unsigned int)kRadixThreads, 0, chained, stream, p);
   }
+  bool chained = true;
+  if (e == cudaSuccess)
+    e = launch_chained(starts_kernel, (unsigned int)(f.rows / kStartsThreads + 1), (unsigned int)kStartsThreads, 0, chained, stream, (const uint32_t*)(ws + g.key[result]), p.n, p.rows,
+                       (uint32_t*)(ws + g.starts), (uint32_t*)(ws + g.counters), (uint32_t)(3 * g.chunks * g.tiles));
   return e == cudaSuccess ? FO_OK : fail(FO_ERR_CUDA, "fo_embed_grad: launch failed: %s", cudaGetErrorString(e));
 }
 
@@ -595,27 +870,40 @@ extern "C" int fo_embed_grad(const FoEmbedGrad* f, void* cuda_stream) {
     return fail(FO_ERR_INVALID_ARG, "fo_embed_grad: a workspace of %llu bytes, aligned to 16, is needed, got %llu", (unsigned long long)g.bytes, (unsigned long long)f->workspace_bytes);
   cudaStream_t stream = (cudaStream_t)cuda_stream;
   int at = 0;
-  if (int rc = g.several ? sort_in_memory(*f, g, stream, at) : sort_in_cluster(*f, g, stream)) return rc;
-  if (f->n_tokens == 0) return FO_OK;
+  if (int rc = g.several ? sort_in_memory(*f, g, stream, at) : sort_by_rows(*f, g, stream)) return rc;
   char* const ws = (char*)f->workspace;
   p.dy = f->dy; p.out = f->out;
   p.key = (const uint32_t*)(ws + g.key[at]); p.pos = (const uint32_t*)(ws + g.pos[at]);
+  p.starts = (const uint32_t*)(ws + g.starts); p.counters = (uint32_t*)(ws + g.counters);
   p.partial = (float*)(ws + g.partial);
-  p.n = f->n_tokens; p.dim = f->dim; p.dy_stride = f->dy_stride;
-  p.rows = (uint32_t)f->rows; p.tiles = g.tiles; p.chunk = g.chunk; p.chunks = g.chunks;
-  p.out_dtype = f->out_dtype; p.accumulate = f->accumulate != 0;
-  p.out_vectors = on_16_bytes(f->out) && f->dim * size_of(f->out_dtype) % 16 == 0;
+  p.dim = f->dim; p.dy_bytes = (uint32_t)(f->dy_stride * size_of(f->dy_dtype)); p.row_bytes = f->dim * size_of(f->out_dtype);
+  p.rows = (uint32_t)f->rows; p.last_token = (uint32_t)(f->n_tokens - 1); p.dealt = !g.several; p.tiles = g.tiles; p.chunk = g.chunk; p.chunks = g.chunks;
   p.factor = (float)(f->scale * factor);
-  const bool vectors = f->dim % 8 == 0 && on_16_bytes(f->dy) && f->dy_stride * size_of(f->dy_dtype) % 16 == 0;
+  const bool vectors = f->dim % 8 == 0 && on_16_bytes(f->dy) && f->dy_stride * size_of(f->dy_dtype) % 16 == 0 && on_16_bytes(f->out);
   void (*kernel)(const SumParams) = nullptr;
-#define X(D) \
-  if (f->dy_dtype == D) kernel = vectors ? sum_kernel<D, true> : sum_kernel<D, false>;
-  X(FO_F32) X(FO_BF16) X(FO_F16)
+  int smem = 0;
+#define Y(D, O, V, P, A) \
+  if (f->dy_dtype == D && f->out_dtype == O && vectors == V && (p.drop.on != 0) == P && (f->accumulate != 0) == A) {      \
+    kernel = sum_kernel<D, O, V, P, A>;                                                                                              \
+    smem = Ring<D, O, V, A>::kBlock;                                                                                                 \
+  }
+#define X(D, O)                                                                                                          \
+  Y(D, O, true, true, true) Y(D, O, true, true, false) Y(D, O, true, false, true) Y(D, O, true, false, false)             \
+  Y(D, O, false, true, true) Y(D, O, false, true, false) Y(D, O, false, false, true) Y(D, O, false, false, false)
+  X(FO_F32, FO_F32) X(FO_F32, FO_BF16) X(FO_F32, FO_F16) X(FO_BF16, FO_F32) X(FO_BF16, FO_BF16) X(FO_BF16, FO_F16) X(FO_F16, FO_F32) X(FO_F16, FO_BF16) X(FO_F16, FO_F16)
 #undef X
-  const unsigned long long tasks = (unsigned long long)g.chunks * g.tiles, blocks = (tasks + kSumThreads / 32 - 1) / (kSumThreads / 32);
-  if (tasks > 0x7FFFFFFFull) return fail(FO_ERR_TOO_LARGE, "fo_embed_grad: %llu tokens of %llu elements exceed one launch", (unsigned long long)f->n_tokens, (unsigned long long)f->dim);
+#undef Y
+  const unsigned long long tasks = (unsigned long long)g.chunks * g.tiles;
   bool chained = true;
-  cudaError_t e = launch_chained(kernel, (unsigned int)blocks, (unsigned int)kSumThreads, 0, chained, stream, p);
-  if (e == cudaSuccess) e = launch_chained(join_kernel, (unsigned int)tasks, (unsigned int)kSumThreads, 0, chained, stream, p);
+  cudaError_t e = cudaSuccess;
+  // (some rings are above the 48 KB that need no word; set at each call: it costs nothing next to the launch)
+  if (smem > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (tasks > 0 && e == cudaSuccess) e = launch_chained(kernel, (unsigned int)((tasks + kSumThreads / 32 - 1) / (kSumThreads / 32)), (unsigned int)kSumThreads, smem, chained, stream, p);
+  if (!f->accumulate && e == cudaSuccess) {
+    ClearParams c = {p.starts, (char*)f->out, p.row_bytes, p.rows, 0, p.dealt, tasks == 0};
+    const unsigned long long per_block = (kClearBytes + p.row_bytes - 1) / p.row_bytes;
+    c.per_block = (uint32_t)(per_block < kClearThreads / 32 ? kClearThreads / 32 : per_block);
+    e = launch_chained(clear_kernel, (p.rows + c.per_block - 1) / c.per_block, (unsigned int)kClearThreads, 0, chained, stream, c);
+  }
   return e == cudaSuccess ? FO_OK : fail(FO_ERR_CUDA, "fo_embed_grad: launch failed: %s", cudaGetErrorString(e));
 }

@@ -16,11 +16,12 @@ int fail(int code, const char* fmt, ...);
 // an element costs 1/8 of a block: with 32 bits from the first block on, the ten rounds of two wide products
 // would cost twice as much, more than the bytes they decide on take at 6.4 TB/s.
 struct Drop {
-  uint32_t key0, key1, off0, off1;
+  uint32_t key[20];  // two per round: an operand of an instruction each, where sums of the seed would take registers in every kernel's loop
+  uint32_t off0, off1;
   const void* dev_offset;  // added to the offset when it is not null
   int32_t dev_bits;        // 32 or 64
-  uint32_t above;          // the least upper half that stays without a look at the lower
-  uint32_t hi, lo;         // T; lo is 0 or a tie needs the second block
+  uint32_t above;          // what a drawn half, shifted up by 16, is greater than where the element stays
+  uint32_t hi, lo;         // T, its upper half in both halves of a word; lo is 0 or a tie needs the second block
   int32_t on;
 };
 
@@ -34,67 +35,74 @@ inline bool make_drop(const FoDropout* f, Drop& d, double& factor) {
   const uint64_t t = (uint64_t)(f->p * 4294967296.0 + 0.5);
   if (t == 0) return true;
   d.on = 1;
-  d.key0 = (uint32_t)f->seed; d.key1 = (uint32_t)(f->seed >> 32);
+  for (uint32_t r = 0; r < 10; ++r) {
+    d.key[2 * r] = (uint32_t)f->seed + r * 0x9E3779B9u;
+    d.key[2 * r + 1] = (uint32_t)(f->seed >> 32) + r * 0xBB67AE85u;
+  }
   d.off0 = (uint32_t)f->offset; d.off1 = (uint32_t)(f->offset >> 32);
   d.dev_offset = f->dev_offset; d.dev_bits = f->dev_offset_bits;
-  d.hi = (uint32_t)(t >> 16); d.lo = (uint32_t)(t & 0xFFFF);
-  d.above = d.hi + (d.lo != 0 ? 1u : 0u);
+  const uint32_t hi = (uint32_t)(t >> 16);
+  d.lo = (uint32_t)(t & 0xFFFF);
+  d.hi = hi | hi << 16;                                                  // (p = 1: lo is 0, not looked at)
+  d.above = (uint32_t)(((uint64_t)hi + (d.lo != 0 && hi != 0xFFFFu ? 1u : 0u)) << 16) - 1u;  // (p = 1: all ones, none stays)
   factor = f->p < 1.0 ? 1.0 / (1.0 - f->p) : 0.0;
   return true;
 }
 
-// the call's own counter, where part of it lies on the device (so that a captured call drops other elements at each replay)
-FO_DEVI void resolve_offset(Drop& d) {
-  if (d.dev_offset == nullptr) return;
+// the call's offset, part of which may lie on the device (so that a captured call drops other elements at each replay)
+FO_DEVI uint2 drop_offset(const Drop& d) {
+  if (d.dev_offset == nullptr) return make_uint2(d.off0, d.off1);
   const long long more = d.dev_bits == 64 ? *(const long long*)d.dev_offset : (long long)*(const int*)d.dev_offset;
   const unsigned long long o = (((unsigned long long)d.off1 << 32) | d.off0) + (unsigned long long)more;
-  d.off0 = (uint32_t)o;
-  d.off1 = (uint32_t)(o >> 32);
+  return make_uint2((uint32_t)o, (uint32_t)(o >> 32));
 }
 
-FO_DEVI uint4 philox(const Drop& d, const uint32_t c0, const uint32_t c1) {
-  uint32_t x0 = c0, x1 = c1, x2 = d.off0, x3 = d.off1, k0 = d.key0, k1 = d.key1;
+FO_DEVI uint4 philox(const Drop& d, const uint2 off, const uint32_t c0, const uint32_t c1) {
+  uint32_t x0 = c0, x1 = c1, x2 = off.x, x3 = off.y;
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const unsigned long long a = (unsigned long long)x0 * 0xD2511F53u, b = (unsigned long long)x2 * 0xCD9E8D57u;
-    x0 = (uint32_t)(b >> 32) ^ x1 ^ k0;
+    x0 = (uint32_t)(b >> 32) ^ x1 ^ d.key[2 * r];
     x1 = (uint32_t)b;
-    x2 = (uint32_t)(a >> 32) ^ x3 ^ k1;
+    x2 = (uint32_t)(a >> 32) ^ x3 ^ d.key[2 * r + 1];
     x3 = (uint32_t)a;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
   }
   return make_uint4(x0, x1, x2, x3);
 }
 
-// Bit j: element 8 * block + j stays.
-FO_DEVI uint32_t keep8(const Drop& d, const unsigned long long block) {
-  const uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32);  // (below 2^61 blocks: the top bit is the second stream's)
-  const uint4 w = philox(d, c0, c1);
-  const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-  uint32_t keep = 0, tie = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t lo = v[j] & 0xFFFFu, hi = v[j] >> 16;
-    keep |= (lo >= d.above ? 1u : 0u) << (2 * j) | (hi >= d.above ? 1u : 0u) << (2 * j + 1);
-    tie |= (lo == d.hi ? 1u : 0u) << (2 * j) | (hi == d.hi ? 1u : 0u) << (2 * j + 1);
-  }
-  if (d.lo != 0 && tie != 0) {  // one element in 2^16
-    const uint4 s = philox(d, c0, c1 | 0x80000000u);
-    const uint32_t u[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t low = (j & 1) != 0 ? u[j / 2] >> 16 : u[j / 2] & 0xFFFFu;
-      if ((tie >> j & 1u) != 0 && low >= d.lo) keep |= 1u << j;
-    }
-  }
-  return keep;
+// The upper halves for the eight elements of a block, two to a word.  A tie, one element in 2^16, is settled here: its half becomes all ones where the
+// element stays and zero where it does not, so that the eight need a shift and two comparisons per pair (`stays`).
+FO_DEVI uint4 settle_ties(const Drop& d, const uint2 off, const uint32_t c0, const uint32_t c1, uint4 w) {
+  const uint4 low = philox(d, off, c0, c1 | 0x80000000u);
+  auto settle = [&](uint32_t& v, const uint32_t u) {
+    if (((v ^ d.hi) & 0xFFFFu) == 0) v = (v & 0xFFFF0000u) | ((u & 0xFFFFu) >= d.lo ? 0xFFFFu : 0u);
+    if ((v ^ d.hi) < 0x10000u) v = (v & 0xFFFFu) | ((u >> 16) >= d.lo ? 0xFFFF0000u : 0u);
+  };
+  settle(w.x, low.x);
+  settle(w.y, low.y);
+  settle(w.z, low.z);
+  settle(w.w, low.w);
+  return w;
 }
-// the same for eight elements from any e on
-FO_DEVI uint32_t keep8_from(const Drop& d, const unsigned long long e) {
-  const uint32_t s = (uint32_t)e & 7u;
-  uint32_t keep = keep8(d, e >> 3) >> s;
-  if (s != 0) keep |= keep8(d, (e >> 3) + 1) << (8 - s);
+FO_DEVI uint4 draw8(const Drop& d, const uint2 off, const unsigned long long block) {
+  const uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32);  // (below 2^61 blocks: the top bit is the second stream's)
+  uint4 w = philox(d, off, c0, c1);
+  if (d.lo != 0) {
+    const uint32_t least = __vminu2(__vminu2(w.x ^ d.hi, w.y ^ d.hi), __vminu2(w.z ^ d.hi, w.w ^ d.hi));
+    if ((least & 0xFFFFu) == 0 || least < 0x10000u) w = settle_ties(d, off, c0, c1, w);
+  }
+  return w;
+}
+FO_DEVI bool stays(const Drop& d, const uint4& w, const int j) {
+  const uint32_t v = j < 2 ? w.x : (j < 4 ? w.y : (j < 6 ? w.z : w.w));
+  return ((j & 1) != 0 ? v : v << 16) > d.above;
+}
+// Bit j: element 8 * block + j stays.
+FO_DEVI uint32_t keep8(const Drop& d, const uint2 off, const unsigned long long block) {
+  const uint4 w = draw8(d, off, block);
+  uint32_t keep = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) keep |= (stays(d, w, j) ? 1u : 0u) << j;
   return keep;
 }
 
