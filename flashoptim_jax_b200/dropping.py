@@ -74,6 +74,9 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset=0, *, residual: Optiona
     optimizer's state, say), read when the kernel runs: a captured call then drops other elements at each replay.  Until the
     backward pass has run it must keep its value.  Differentiable in x and residual (once); by hand, the gradient of x is
     `dropout(dy, p, seed, offset)` and that of the residual is dy."""
+    y = _lib.host().dropout(x, p, seed, offset, residual)  # None: something to differentiate or convert first, or an error to report
+    if y is not None:
+        return y
     require_cuda(x, "x")
     if x.dtype not in DTYPE_CODE:
         raise ValueError(f"dropout takes float32, bfloat16 or float16, got {dtype_name(x.dtype)}")

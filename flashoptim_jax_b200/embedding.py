@@ -90,6 +90,10 @@ def embed(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, ecc: Op
     `ecc` fp32; `dtype` may ask for either.  `ids`: int32 or int64.  A negative id is no token: its row is 0 and it has no part in the
     gradient.  An id behind the last row cannot be reported without waiting for the GPU: its row is NaN, which the loss shows.
     Differentiable in the table (once): the gradient is `embed_grad`'s, in the table's dtype."""
+    if dtype is None:
+        out = _lib.host().embed(table, ids, ecc, scale, p, seed, offset)  # None: something to differentiate or convert first, or an error to report
+        if out is not None:
+            return out
     require_cuda(table, "table")
     if table.dim() != 2 or table.dtype not in DTYPE_CODE:
         raise ValueError(f"table must be a float32, bfloat16 or float16 matrix, got shape {tuple(table.shape)}, {dtype_name(table.dtype)}")
@@ -120,6 +124,10 @@ def embed_grad(dy: torch.Tensor, ids: torch.Tensor, rows: int, *, scale: float =
     bits), rounded once; rows without a token are 0.  Into `out` where it is given (a leaf of `Zero1Optimizer.grads`, say); with `accumulate` the sums
     are added to what `out` holds (the gradient that the output head of a tied model left there, or an earlier micro-batch's), and rows without a
     token are neither read nor written."""
+    if dtype is None:
+        grad = _lib.host().embed_grad(dy, ids, rows, scale, p, seed, offset, out, accumulate)  # None: something to convert first, or an error to report
+        if grad is not None:
+            return grad
     require_cuda(dy, "dy")
     _check_ids(ids, dy.device)
     if dy.dtype not in DTYPE_CODE:

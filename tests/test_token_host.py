@@ -110,9 +110,9 @@ def test_workspace_sizes():
         return out.value
 
     assert need(0, 8, 5) == 0 and need(5, 0, 5) == 0
-    # keys and positions at least; partial sums of one row at either end of a chunk stay a few megabytes whatever the sizes
+    # keys and positions, and where each row's tokens begin; partial sums of one row at either end of a chunk stay a few megabytes whatever the sizes
     for rows, dim, n in ((1, 1, 1), (100, 7, 33), (50257, 768, 16384), (128256, 4096, 1 << 20), (2**31 - 2, 8, 2**31 - 2), (8, 2**24 - 1, 4)):
-        assert 8 * n <= need(rows, dim, n) <= 17 * n + 8 * dim + (64 << 20), (rows, dim, n)
+        assert 8 * n <= need(rows, dim, n) <= 17 * n + 4 * rows + 8 * dim + (64 << 20), (rows, dim, n)
     assert lib.fo_embed_grad_workspace(2**31, 8, 1, ctypes.byref(ctypes.c_uint64())) == 4
     assert lib.fo_embed_grad_workspace(8, 8, 1, None) == 1
 
