@@ -4,7 +4,7 @@
 
 namespace fo {
 
-constexpr int kEmbedThreads = 256;
+constexpr int kEmbedThreads = 128;
 
 struct EmbedParams {
   const void* table;
@@ -13,6 +13,7 @@ struct EmbedParams {
   void* out;
   unsigned long long n_tokens, rows, dim;
   unsigned long long row_stride, ecc_stride;  // elements
+  uint32_t tiles;  // of 256 columns
   int32_t ids_bits, out_f32;
   float factor;  // scale, and 1 / (1 - p)
   Drop drop;
@@ -32,12 +33,6 @@ struct EccOct {
     return 0;
   }
 };
-
-template <int DT, int ECC>
-FO_DEVI float weight(const void* table, const void* ecc, const unsigned long long i, const unsigned long long i_ecc) {
-  if constexpr (ECC == 0) return load1<DT>(table, i);
-  else return fast::reconstruct<DT, ECC>(((const unsigned short*)table)[i], ECC == 16 ? (int)((const short*)ecc)[i_ecc] : (int)((const signed char*)ecc)[i_ecc]);
-}
 
 // A negative id is no token: zeros.  An id behind the last row reads nothing: a row of NaN, seen in the loss.
 FO_DEVI float without_row(const long long id) { return id < 0 ? 0.0f : __int_as_float(0x7FC00000); }
@@ -110,56 +105,66 @@ __global__ void __launch_bounds__(kEmbedThreads) embed_kernel(const __grid_const
   }
 }
 
-// Any width, stride and alignment: 256 neighbouring results per warp, which may lie in several rows, neighbours in neighbouring lanes; each lane draws
-// for eight neighbours and hands them on.
-template <int DT, int ECC>
+// Any width, stride and alignment: a warp per 256 columns of a token, every 32nd of them to a lane, so that neighbours lie in neighbouring lanes.  The id and
+// all addresses are the warp's, worked out once; each lane draws for eight neighbours and hands them on.
+template <int DT, int ECC, bool F32>
 __global__ void __launch_bounds__(kEmbedThreads) embed_any_kernel(const __grid_constant__ EmbedParams p) {
   chain_wait();
   chain_release();
   const Drop& d = p.drop;
-  const uint2 off = drop_offset(d);
   const int lane = threadIdx.x & 31;
-  const unsigned long long total = p.n_tokens * p.dim, first = ((unsigned long long)blockIdx.x * kEmbedThreads + (threadIdx.x & ~31u)) * 8;
-  unsigned long long n, c;
-  if (first + 256 < 0xFFFFFFFFull && p.dim <= 0xFFFFFFFFull) {
-    n = (uint32_t)(first + lane) / (uint32_t)p.dim;
-    c = (uint32_t)(first + lane) - (uint32_t)n * (uint32_t)p.dim;
-  } else {
-    n = (first + lane) / p.dim;
-    c = first + lane - n * p.dim;
-  }
-  long long id[8];
-  unsigned long long col[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    col[j] = c;
-    id[j] = first + j * 32 + lane < total ? id_at(p.ids, p.ids_bits, n) : -1;
-    for (c += 32; c >= p.dim; c -= p.dim) ++n;
-  }
+  const unsigned long long task = (unsigned long long)blockIdx.x * (kEmbedThreads / 32) + threadIdx.x / 32;
+  const unsigned long long n = task / p.tiles;
+  if (n >= p.n_tokens) return;
+  const uint32_t c0 = (uint32_t)(task - n * p.tiles) * 256;
+  const int count = (int)min(256u, (uint32_t)p.dim - c0) - lane;  // columns from the lane's first one on
+  const long long id = id_at(p.ids, p.ids_bits, n);
+  const bool named = id >= 0 && (unsigned long long)id < p.rows;
+  const unsigned long long row = named ? (unsigned long long)id : 0ull;
+  const char* const w = (const char*)p.table + (row * p.row_stride + c0 + lane) * size_of(DT);
+  const char* const e = (const char*)p.ecc + (row * p.ecc_stride + c0 + lane) * (ECC / 8);
   float v[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    v[j] = id[j] < 0 || (unsigned long long)id[j] >= p.rows
-               ? without_row(id[j])
-               : weight<DT, ECC>(p.table, p.ecc, (unsigned long long)id[j] * p.row_stride + col[j], (unsigned long long)id[j] * p.ecc_stride + col[j]);
-  const uint32_t mine = d.on ? keep8(d, off, first / 8 + lane) : 0xFFu;
+  int code[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const unsigned long long e = first + j * 32 + lane;
-    v[j] = (__shfl_sync(~0u, mine, j * 4 + lane / 8) >> (lane & 7) & 1u) != 0 ? fmul(v[j], p.factor) : 0.0f;
-    if (e >= total) continue;
-    if (DT == FO_F32 || p.out_f32) store1<FO_F32>(p.out, e, v[j]);
-    else store1<DT>(p.out, e, v[j]);
+    v[j] = without_row(id);
+    if (named && j * 32 < count) {
+      v[j] = __uint_as_float(DT == FO_F32 ? ((const uint32_t*)w)[j * 32] : ((const unsigned short*)w)[j * 32]);
+      if constexpr (ECC == 16) code[j] = ((const short*)e)[j * 32];
+      if constexpr (ECC == 8) code[j] = ((const signed char*)e)[j * 32];
+    }
+  }
+  const unsigned long long e0 = n * p.dim + c0;
+  uint32_t low = 0xFFu, high = 0xFFu;  // the warp's 256 columns lie in 32 or 33 blocks of eight
+  if (d.on) {
+    const uint2 off = drop_offset(d);
+    low = keep8(d, off, (e0 >> 3) + lane);
+    if ((e0 & 7) != 0) high = keep8(d, off, (e0 >> 3) + 32);
+  }
+  char* const to = (char*)p.out + (e0 + lane) * (F32 ? 4 : size_of(DT));
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (named) {
+      if constexpr (ECC != 0) v[j] = fast::reconstruct<DT, ECC>(__float_as_uint(v[j]), code[j]);
+      else if constexpr (DT != FO_F32) v[j] = Lp<DT>::to_f32(__float_as_uint(v[j]));
+    }
+    v[j] = fmul(v[j], p.factor);
+    if (d.on) {
+      const uint32_t at = ((uint32_t)e0 & 7u) + j * 32 + lane;
+      const uint32_t bits = __shfl_sync(~0u, low, (at >> 3) & 31);
+      if (((at >= 256 ? high : bits) >> (at & 7) & 1u) == 0) v[j] = 0.0f;
+    }
+    if (j * 32 < count) store1<F32 ? FO_F32 : DT>(to, j * 32, v[j]);
   }
 }
 
 template <int DT, int ECC>
 static int launch_embed(const EmbedParams& p, const bool vectors, cudaStream_t stream) {
-  constexpr int kOcts = 2;
-  const unsigned long long octs = vectors ? p.n_tokens * (p.dim / 8) : (p.n_tokens * p.dim + 7) / 8;
-  const unsigned long long per_block = (unsigned long long)kEmbedThreads * (vectors ? kOcts : 1), blocks = (octs + per_block - 1) / per_block;
+  const unsigned long long octs = p.n_tokens * (p.dim / 8), warps = p.n_tokens * p.tiles;
+  constexpr int kOcts = 4;
+  const unsigned long long per_block = vectors ? kEmbedThreads * kOcts : kEmbedThreads / 32, blocks = ((vectors ? octs : warps) + per_block - 1) / per_block;
   if (blocks > 0x7FFFFFFFull) return fail(FO_ERR_TOO_LARGE, "fo_embed: %llu tokens of %llu elements exceed one launch", p.n_tokens, p.dim);
-  void (*kernel)(const EmbedParams) = embed_any_kernel<DT, ECC>;
+  void (*kernel)(const EmbedParams) = p.out_f32 ? embed_any_kernel<DT, ECC, true> : embed_any_kernel<DT, ECC, DT == FO_F32>;
   if (vectors) kernel = octs < 0xFFFF0000ull ? embed_kernel<DT, ECC, uint32_t, kOcts> : embed_kernel<DT, ECC, unsigned long long, kOcts>;
   bool chained = true;
   const cudaError_t e = launch_chained(kernel, (unsigned int)blocks, (unsigned int)kEmbedThreads, 0, chained, stream, p);
@@ -191,6 +196,7 @@ extern "C" int fo_embed(const FoEmbed* f, void* stream) {
   p.table = f->table; p.ecc = f->ecc; p.ids = f->ids; p.out = f->out;
   p.n_tokens = f->n_tokens; p.rows = f->rows; p.dim = f->dim;
   p.row_stride = f->row_stride; p.ecc_stride = f->ecc_stride;
+  p.tiles = (uint32_t)((p.dim + 255) / 256);
   p.ids_bits = f->ids_bits;
   p.out_f32 = f->out_dtype == FO_F32;
   p.factor = (float)((double)f->scale * factor);
