@@ -15,7 +15,8 @@ constexpr int kSms = 148;
 // ---- sizes and the workspace ----------------------------------------------------------------------------------------
 constexpr int kTileCols = 256;     // columns of a warp: eight per lane
 constexpr int kSumThreads = 256, kSumBlocksPerSm = 3;
-constexpr int kLeastChunk = 8;     // tokens
+constexpr int kLeastChunk = 4;     // tokens
+constexpr uint32_t kFewTokens = 64;  // up to so many take one launch and no workspace
 constexpr int kSumWarps = kSms * kSumBlocksPerSm * kSumThreads / 32;  // wanted: all of them resident at once
 
 // The sort by rows, in one launch or two: 128 blocks, a 16-bit counter per row and warp.
@@ -23,25 +24,35 @@ constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kSortRows = 2048;                      // of a block, at most
 constexpr uint32_t kSortBlocks = 128;
 constexpr unsigned long long kSortMost = 65536;      // tokens
-constexpr unsigned long long kSortAlone = 4096;  // of which up to so many take one launch
-// The sort over several launches: tiles of 4096 tokens, digits of at most nine bits.
+constexpr unsigned long long kSortAlone = 8192;  // of which up to so many take one launch
+constexpr int kSortSmem = 220 * 1024;
+static_assert(kSortRows == 2 * kSortThreads && (kSortWarps * 2 + 4) * (kSortRows + 2) <= kSortSmem && kSortMost <= 65536, "two rows a thread, shared memory, places that fit the counters");
+// The sort by digits, over several launches: tiles of 4096 tokens, digits of at most nine bits.
 constexpr int kDigitMax = 9, kBinsMax = 1 << kDigitMax;
 constexpr int kRadixThreads = 512, kRadixRounds = 8, kRadixTile = kRadixThreads * kRadixRounds;
 
 struct GradPlan {
-  bool several;  // the sort takes several launches
+  bool alone, several;  // the sort takes one launch, or several per digit; otherwise two
   uint32_t tiles, chunk, chunks;
-  uint32_t blocks;  // of such a sort
+  uint32_t blocks;  // of a sort by digits
+  unsigned int sort_smem;
   unsigned long long key[2], pos[2], starts, counters, hist, total, partial, bytes;  // offsets in the workspace
 };
 
 static GradPlan plan_of(const unsigned long long rows, const unsigned long long dim, const unsigned long long n) {
   GradPlan g = {};
+  if (n <= kFewTokens) {
+    g.tiles = (uint32_t)((dim + kTileCols - 1) / kTileCols);
+    return g;
+  }
   g.several = n > kSortMost || rows >= (unsigned long long)kSortBlocks * kSortRows;
+  const unsigned long long width = (rows / kSortBlocks + 2) & ~1ull, lists = 4 * ((n + kSortThreads - 1) / kSortThreads * kSortThreads);
+  g.alone = !g.several && n <= kSortAlone && (kSortWarps * 2 + 4) * width + lists <= kSortSmem;
+  g.sort_smem = g.several ? 0u : (unsigned int)((kSortWarps * 2 + 4) * width + (g.alone ? lists : 0));
   g.tiles = (uint32_t)((dim + kTileCols - 1) / kTileCols);
   unsigned long long chunk = (n * g.tiles + kSumWarps - 1) / kSumWarps;
   if (chunk < kLeastChunk) chunk = kLeastChunk;
-  if (chunk > n && n > 0) chunk = n;
+  if (chunk > n) chunk = n;
   g.chunk = (uint32_t)chunk;
   g.chunks = (uint32_t)((n + chunk - 1) / chunk);
   g.blocks = (uint32_t)((n + kRadixTile - 1) / kRadixTile);
@@ -52,13 +63,13 @@ static GradPlan plan_of(const unsigned long long rows, const unsigned long long 
     return here;
   };
   const unsigned long long dealt = (n + 2 * kSortThreads - 1) / (2 * kSortThreads) * (2 * kSortThreads);
-  for (int i = 0; i < (n > kSortAlone || g.several ? 2 : 1); ++i) {
+  for (int i = 0; i < (g.alone ? 1 : 2); ++i) {
     g.key[i] = take(4 * dealt);
     g.pos[i] = take(4 * dealt);
   }
   g.starts = take(4 * (rows + 1));
   g.counters = take(12ull * g.chunks * g.tiles);
-  if (!g.several && n > kSortAlone) g.hist = take(4ull * kSortBlocks * (kSortMost / (2 * kSortThreads)));
+  if (!g.several && !g.alone) g.hist = take(4ull * kSortBlocks * (kSortMost / (2 * kSortThreads)));
   if (g.several) {
     g.hist = take(4ull * kBinsMax * g.blocks);
     g.total = take(4ull * kBinsMax);
@@ -70,7 +81,7 @@ static GradPlan plan_of(const unsigned long long rows, const unsigned long long 
 
 // ---- (1) the sort ----------------------------------------------------------------------------------------------------
 // Ids that name no row sort behind all rows.
-FO_DEVI uint32_t key_of(const long long id, const uint32_t rows) { return id < 0 || id >= (long long)rows ? rows : (uint32_t)id; }
+FO_DEVI uint32_t key_of(const long long id, const uint32_t rows) { return (unsigned long long)id < rows ? (uint32_t)id : rows; }
 
 // Zeros from a to b (elements of 2 or 4 bytes) by one warp.
 FO_DEVI void clear_bytes(char* a, char* const b, const int lane) {
@@ -140,11 +151,13 @@ struct SortParams {
 __host__ __device__ inline uint32_t rows_before(const uint32_t block, const uint32_t rows) { return block * (rows / kSortBlocks) + min(block, rows % kSortBlocks); }
 FO_DEVI uint32_t slot_of(const uint32_t row, const uint32_t rows) { return rows_before(row % kSortBlocks, rows) + row / kSortBlocks; }
 
-// Up to kSortMost tokens, in one launch and without a word between its blocks: each block has 1 / 128 of the rows.  It reads all ids (from the L2: at 64
+// Up to kSortAlone tokens, in one launch and without a word between its blocks: each block has 1 / 128 of the rows.  It reads all ids (from the L2: at 64
 // bytes a clock 16384 of them take 1 us), counts those of blocks in front of it, which is where its tokens begin in the order, and
-// those of each of its rows, warp by warp, each warp having the tokens behind those of the one before; then it walks over the ids again and puts its
-// tokens in their places.  Eight blocks that sorted by digits through the shared memory of a cluster took 12.4 us for 8192 tokens, mostly waiting
+// those of each of its rows, warp by warp, each warp having the tokens behind those of the one before and keeping a list of the block's among them; then
+// each warp puts its list in place.  Eight blocks that sorted by digits through the shared memory of a cluster took 12.4 us for 8192 tokens, mostly waiting
 // for one another.  Loops stay loops: unrolled, their code took longer to fetch than to run.
+constexpr int kHitBits = 10;  // of a token's number within its warp's, and of its rank there: 32 warps x 2^10 = 32768 tokens
+static_assert(kSortAlone <= (unsigned long long)kSortWarps << kHitBits && kSortRows <= 1 << (32 - 2 * kHitBits), "a hit is one word");
 __global__ void __launch_bounds__(kSortThreads) sort_kernel(const __grid_constant__ SortParams p) {
   chain_wait();
   chain_release();
@@ -155,35 +168,35 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const __grid_constan
   const uint32_t me = blockIdx.x, slots = rows_before(me, p.rows), mine = rows_before(me + 1, p.rows) - slots;
   const uint32_t width = (p.rows / kSortBlocks + 2) & ~1u;  // of a warp's counters
   uint32_t* const first = (uint32_t*)(sort_mem + (size_t)kSortWarps * width * 2);  // [row]
+  const uint32_t rounds = (p.n + kSortThreads - 1) / kSortThreads;
+  uint32_t* const list = first + width + warp * rounds * 32;  // row << 20 | rank among the warp's tokens of the row << 10 | token
   for (uint32_t i = threadIdx.x; i < kSortWarps * width / 2; i += kSortThreads) ((uint32_t*)counts)[i] = 0;
   for (uint32_t i = me * kSortThreads + threadIdx.x; i < p.n_counters; i += gridDim.x * kSortThreads) p.counters[i] = 0;
-  const uint32_t rounds = (p.n + kSortThreads - 1) / kSortThreads;
   const uint32_t i0 = warp * rounds * 32 + lane;
+  unsigned short* const my_counts = counts + warp * width;
   constexpr int kAtOnce = 4;
-  uint32_t below = 0;
+  uint32_t below = 0, hits = 0;
   __syncthreads();
-  // f(key, rank among the warp's tokens of its row, token) for this block's tokens
-  auto walk = [&](auto f) {
 #pragma unroll 1
-    for (uint32_t r0 = 0; r0 < rounds; r0 += kAtOnce) {
-      uint32_t key[kAtOnce];
+  for (uint32_t r0 = 0; r0 < rounds; r0 += kAtOnce) {
+    uint32_t key[kAtOnce];
 #pragma unroll
-      for (int r = 0; r < kAtOnce; ++r) {
-        const uint32_t i = i0 + (r0 + r) * 32;
-        key[r] = r0 + r < rounds && i < p.n ? key_of(id_at(p.ids, p.ids_bits, i), p.rows) : p.rows;
-      }
-#pragma unroll
-      for (int r = 0; r < kAtOnce; ++r) {
-        const uint32_t block = key[r] % kSortBlocks;
-        const bool in = key[r] < p.rows && block == me;
-        below += key[r] < p.rows && block < me ? 1u : 0u;
-        if (!__any_sync(~0u, in)) continue;
-        const uint32_t rank = rank_in_warp(key[r] / kSortBlocks, in, p.row_bits, counts + warp * width, lane);
-        if (in) f(key[r], rank, i0 + (r0 + r) * 32);
-      }
+    for (int r = 0; r < kAtOnce; ++r) {
+      const uint32_t i = i0 + (r0 + r) * 32;
+      key[r] = r0 + r < rounds && i < p.n ? key_of(id_at(p.ids, p.ids_bits, i), p.rows) : p.rows;
     }
-  };
-  walk([](uint32_t, uint32_t, uint32_t) {});
+#pragma unroll
+    for (int r = 0; r < kAtOnce; ++r) {
+      const uint32_t block = key[r] < p.rows ? key[r] % kSortBlocks : kSortBlocks;
+      below += block < me ? 1u : 0u;
+      const bool in = block == me;
+      const uint32_t found = __ballot_sync(~0u, in);
+      if (found == 0) continue;
+      const uint32_t rank = rank_in_warp(key[r] / kSortBlocks, in, p.row_bits, my_counts, lane);
+      if (in) list[hits + __popc(found & ((1u << lane) - 1u))] = key[r] / kSortBlocks << 2 * kHitBits | rank << kHitBits | ((r0 + r) * 32 + lane);
+      hits += __popc(found);
+    }
+  }
   uint32_t before, all;
   scan_block(below, warp_sums, before);
   // Per row: the warps' counts to places within the row, and its tokens; two rows a thread, neighbours.
@@ -208,13 +221,12 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const __grid_constan
   }
   if (me == kSortBlocks - 1 && threadIdx.x == 0) p.starts[p.rows] = before + all;
   __syncthreads();
-  // the counters now say where the warp's tokens begin: counting on gives each its place
-  walk([&](const uint32_t key, const uint32_t rank, const uint32_t i) {
-    const uint32_t to = first[key / kSortBlocks] + rank;
-    if (to >= p.n) return;  // (ids that another stream changed between the walks)
-    p.key_out[to] = key;
-    p.pos_out[to] = i;
-  });
+  for (uint32_t h = lane; h < hits; h += 32) {
+    const uint32_t hit = list[h], row = hit >> 2 * kHitBits;
+    const uint32_t to = first[row] + my_counts[row] + (hit >> kHitBits & ((1u << kHitBits) - 1u));
+    p.key_out[to] = row * kSortBlocks + me;
+    p.pos_out[to] = warp * rounds * 32 + (hit & ((1u << kHitBits) - 1u));
+  }
 }
 
 // More tokens than kSortAlone: two launches.  In the first, each block deals its 2048 tokens out to 128 piles by id % 128, each pile in the order of the
@@ -668,27 +680,34 @@ __global__ void __launch_bounds__(kSumThreads, kSumBlocksPerSm) sum_kernel(const
   }
   float sum[8] = {};
   bool any = false;  // a row began in this chunk
+  // Four tokens at a time: single ones cost a third more instructions, and with the draws of dropout in it, the loop unrolled over eight outgrew
+  // the instruction cache.
+  static_assert(kStages % 4 == 0 && kStages <= 8, "a group of four lies in stages 0-3 or 4-7");
 #pragma unroll 1
   for (uint32_t here = first; here < end; here += 32) {
     next_key = here + 32 + lane < end ? p.key[here + 32 + lane] : 0u;
     next_pos = here + 32 + lane < end ? p.pos[here + 32 + lane] : 0u;
 #pragma unroll 1
-    for (uint32_t k0 = 0; k0 < 32; k0 += kStages) {
-      if (k0 == 32 - kStages) next_heads = heads_of(next_key, __shfl_sync(~0u, key, 31));
+    for (uint32_t k0 = 0; k0 < 32; k0 += 4) {
+      if (here + k0 >= end) break;
+      if (k0 == (kStages == 8 ? 24 : 28)) next_heads = heads_of(next_key, __shfl_sync(~0u, key, 31));
+      const uint32_t half = kStages == 8 ? k0 & 4u : 0u;
+      unsigned char* const group = ring + half * R::kStage;
 #pragma unroll
-      for (int s = 0; s < kStages; ++s) {
+      for (int s = 0; s < 4; ++s) {
         const uint32_t k = k0 + s, a = k + kStages - 1;
         if (here + k >= end) break;
         copy_wait<kStages - 2>();
         if constexpr (!VECTORS) __syncwarp();  // the other lanes' copies are there, and the stage that is filled next has been read
         const uint32_t ahead = __shfl_sync(~0u, a < 32 ? pos : next_pos, a & 31);
-        if (here + a < end) fetch(a, ahead, (s + kStages - 1) % kStages);
+        // the stage that is filled next: the one behind, of this group or the last of the other
+        if (here + a < end) fetch(a, ahead, kStages == 8 ? (s == 0 ? (int)(half ^ 4u) + 3 : (int)half + s - 1) : (s + 3) % 4);
         copy_commit();
         const uint32_t at = DROP || !VECTORS ? __shfl_sync(~0u, pos, k) : 0u;
         const unsigned long long e0 = at * p.dim + c0;
         uint4 w = {};
         if constexpr (DROP && VECTORS) w = draw8(p.drop, off, (e0 >> 3) + lane);
-        const unsigned char* const stage = ring + s * R::kStage;
+        const unsigned char* const stage = group + s * R::kStage;
         if ((heads >> k & 1u) != 0) {  // (the same for the whole warp)
           if (opened) put8(piece_at(p, chunk, false, tile, lane), sum);
           else if (any) write_row<OT, VECTORS>(out + row * p.row_bytes + lane * kLaneOut, count, sum);
@@ -706,7 +725,8 @@ __global__ void __launch_bounds__(kSumThreads, kSumBlocksPerSm) sum_kernel(const
         Tile<DT, VECTORS>::get(stage, from + (unsigned long long)at * p.dy_bytes, lane, v);
         if constexpr (DROP && VECTORS) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = stays(p.drop, w, j) ? v[j] : 0.0f;
+          for (int j = 0; j < 8; ++j)
+            if (stays(p.drop, w, j)) sum[j] = __fmaf_rn(v[j], p.factor, sum[j]);
         } else if constexpr (DROP) {  // the warp's 256 columns lie in 32 or 33 blocks of eight
           const uint32_t skew = (uint32_t)e0 & 7u;
           const uint32_t low = keep8(p.drop, off, (e0 >> 3) + lane), high = skew != 0 ? keep8(p.drop, off, (e0 >> 3) + 32) : 0u;
@@ -714,13 +734,13 @@ __global__ void __launch_bounds__(kSumThreads, kSumBlocksPerSm) sum_kernel(const
           for (int j = 0; j < 8; ++j) {
             const uint32_t e = skew + j * 32 + lane;
             const uint32_t bits = __shfl_sync(~0u, low, (e >> 3) & 31);
-            v[j] = ((e >= 256 ? high : bits) >> (e & 7) & 1u) != 0 ? v[j] : 0.0f;
+            if (((e >= 256 ? high : bits) >> (e & 7) & 1u) != 0) sum[j] = __fmaf_rn(v[j], p.factor, sum[j]);
           }
-        }
+        } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum[j] = __fmaf_rn(v[j], p.factor, sum[j]);
+          for (int j = 0; j < 8; ++j) sum[j] = __fmaf_rn(v[j], p.factor, sum[j]);
+        }
       }
-      if (here + k0 + kStages >= end) break;
     }
     key = next_key;
     pos = next_pos;
@@ -748,11 +768,9 @@ struct ClearParams {
   unsigned long long row_bytes;
   uint32_t rows, per_block;
   int32_t dealt;  // starts is in the order of slot_of, not of the rows
-  int32_t wait;   // for the launch in front; otherwise that one has waited for the sort
 };
 __global__ void __launch_bounds__(kClearThreads) clear_kernel(const __grid_constant__ ClearParams p) {
-  if (p.wait) chain_wait();
-  chain_release();
+  chain_release();  // (no wait: the sums in front have waited for the sort)
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
   const uint32_t r0 = blockIdx.x * p.per_block, r1 = min(r0 + p.per_block, p.rows);
   for (uint32_t r = r0 + warp; r < r1; r += kClearThreads / 32) {
@@ -763,6 +781,140 @@ __global__ void __launch_bounds__(kClearThreads) clear_kernel(const __grid_const
     }
   }
   chain_end();
+}
+
+// ---- a handful of tokens, in one launch -------------------------------------------------------------------------------
+// Every block reads all ids.  A warp per token and 256 columns sees whether its token is the first with its id, and then adds up the rows of all that
+// have it, in their order; the blocks behind clear the rows that none names.  Bound by launching and by the latency of ids and rows, which the three
+// launches above pay several times (33 tokens of 1024 columns into 8192 rows, fp32: 11.5 us).  A row of k tokens takes k / 4 trips to memory, so
+// it ends at 64.
+struct FewParams {
+  const void* dy;
+  const void* ids;
+  char* out;
+  unsigned long long dim, row_bytes, dy_bytes;
+  uint32_t n, rows, tiles, token_blocks, clear_rows;
+  int32_t ids_bits, out_dtype, accumulate;
+  float factor;
+  Drop drop;
+};
+template <int DT, bool VECTORS>
+__global__ void __launch_bounds__(kSumThreads) few_kernel(const __grid_constant__ FewParams p) {
+  chain_wait();
+  chain_release();
+  extern __shared__ uint32_t named[];  // a bit per row of the block
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+  uint32_t key[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) key[h] = h * 32 + lane < p.n ? key_of(id_at(p.ids, p.ids_bits, h * 32 + lane), p.rows) : p.rows;
+  if (blockIdx.x >= p.token_blocks) {
+    const uint32_t r0 = (blockIdx.x - p.token_blocks) * p.clear_rows, r1 = min(r0 + p.clear_rows, p.rows);
+    for (uint32_t i = threadIdx.x; i < (r1 - r0 + 31) / 32; i += kSumThreads) named[i] = 0;
+    __syncthreads();
+    if (warp == 0) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (key[h] >= r0 && key[h] < r1) atomicOr(&named[(key[h] - r0) / 32], 1u << ((key[h] - r0) & 31));
+    }
+    __syncthreads();
+    for (uint32_t r = r0 + warp; r < r1; r += kSumThreads / 32)
+      if ((named[(r - r0) / 32] >> ((r - r0) & 31) & 1u) == 0) clear_bytes(p.out + r * p.row_bytes, p.out + (r + 1) * p.row_bytes, lane);
+    return;
+  }
+  const uint32_t task = blockIdx.x * (kSumThreads / 32) + warp, token = task / p.tiles, tile = task - token * p.tiles;
+  if (token >= p.n) return;
+  const uint32_t mine_low = __shfl_sync(~0u, key[0], token & 31), mine_high = __shfl_sync(~0u, key[1], token & 31), row = token < 32 ? mine_low : mine_high;
+  if (row >= p.rows) return;
+  const uint32_t same_low = __ballot_sync(~0u, key[0] == row), same_high = __ballot_sync(~0u, key[1] == row);
+  unsigned long long same = (unsigned long long)same_high << 32 | same_low;
+  if ((same & ((1ull << token) - 1ull)) != 0) return;  // another has it
+  const uint2 off = drop_offset(p.drop);
+  const unsigned long long c0 = (unsigned long long)tile * kTileCols;
+  const int columns = p.dim - c0 < kTileCols ? (int)(p.dim - c0) : kTileCols, count = columns - (VECTORS ? lane * 8 : lane);
+  const char* const from = (const char*)p.dy + (c0 + (VECTORS ? lane * 8 : lane)) * size_of(DT);
+  constexpr int kAhead = 4;
+  float sum[8] = {};
+  while (same != 0) {
+    float v[kAhead][8];
+    uint32_t at[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      at[k] = same != 0 ? (uint32_t)__ffsll((long long)same) - 1u : ~0u;
+      same &= same - 1ull;
+      const char* const x = from + at[k] * p.dy_bytes;
+      if (at[k] == ~0u) continue;
+      if constexpr (VECTORS) {
+        Oct<DT> o;
+        if (count > 0) {
+          o.load(x);
+          o.get(v[k]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j * 32 < count) v[k][j] = load1<DT>(x, j * 32);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (at[k] == ~0u) break;
+      const unsigned long long e0 = at[k] * p.dim + c0;
+      uint32_t low = 0xFFu, high = 0xFFu;
+      if (p.drop.on) {
+        low = keep8(p.drop, off, (e0 >> 3) + lane);
+        if ((e0 & 7) != 0) high = keep8(p.drop, off, (e0 >> 3) + 32);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        uint32_t keep = low >> j;
+        if constexpr (!VECTORS) {
+          const uint32_t e = ((uint32_t)e0 & 7u) + j * 32 + lane, bits = __shfl_sync(~0u, low, (e >> 3) & 31);
+          keep = (e >= 256 ? high : bits) >> (e & 7);
+        }
+        if (!p.drop.on || (keep & 1u) != 0) sum[j] = __fmaf_rn(v[k][j], p.factor, sum[j]);
+      }
+    }
+  }
+  auto write = [&](auto tag) {
+    constexpr int OT = decltype(tag)::value;
+    char* const to = p.out + row * p.row_bytes + (c0 + (VECTORS ? lane * 8 : lane)) * size_of(OT);
+    if (p.accumulate) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        constexpr int kStep = VECTORS ? 1 : 32;
+        if (VECTORS ? count > 0 : j * 32 < count) sum[j] = fadd(load1<OT>(to, j * kStep), sum[j]);
+      }
+    }
+    write_row<OT, VECTORS>(to, count, sum);
+  };
+  if (p.out_dtype == FO_F32) write(std::integral_constant<int, FO_F32>{});
+  else if (p.out_dtype == FO_BF16) write(std::integral_constant<int, FO_BF16>{});
+  else write(std::integral_constant<int, FO_F16>{});
+}
+
+static int few_tokens(const FoEmbedGrad& f, const SumParams& s, const bool vectors, cudaStream_t stream) {
+  FewParams p = {};
+  p.dy = f.dy; p.ids = f.ids; p.out = (char*)f.out;
+  p.dim = f.dim; p.row_bytes = s.row_bytes; p.dy_bytes = s.dy_bytes;
+  p.n = (uint32_t)f.n_tokens; p.rows = s.rows; p.tiles = s.tiles;
+  p.ids_bits = f.ids_bits; p.out_dtype = f.out_dtype; p.accumulate = f.accumulate != 0;
+  p.factor = s.factor; p.drop = s.drop;
+  p.token_blocks = (p.n * p.tiles + kSumThreads / 32 - 1) / (kSumThreads / 32);
+  unsigned int grid = p.token_blocks;
+  if (!f.accumulate) {
+    const unsigned long long per_block = (kClearBytes + s.row_bytes - 1) / s.row_bytes;
+    p.clear_rows = (uint32_t)(per_block < kSumThreads / 32 ? kSumThreads / 32 : per_block);
+    grid += (p.rows + p.clear_rows - 1) / p.clear_rows;
+  }
+  if (grid == 0) return FO_OK;
+  void (*kernel)(const FewParams) = nullptr;
+#define X(D) \
+  if (f.dy_dtype == D) kernel = vectors ? few_kernel<D, true> : few_kernel<D, false>;
+  X(FO_F32) X(FO_BF16) X(FO_F16)
+#undef X
+  bool chained = true;
+  const cudaError_t e = launch_chained(kernel, grid, (unsigned int)kSumThreads, (int)((p.clear_rows + 31) / 32 * 4), chained, stream, p);
+  return e == cudaSuccess ? FO_OK : fail(FO_ERR_CUDA, "fo_embed_grad: launch failed: %s", cudaGetErrorString(e));
 }
 
 static int sizes_ok(const char* who, uint64_t rows, uint64_t dim, uint64_t n) {
@@ -785,29 +937,25 @@ static int sort_by_rows(const FoEmbedGrad& f, const GradPlan& g, cudaStream_t st
   uint32_t *const key = (uint32_t*)(ws + g.key[0]), *const pos = (uint32_t*)(ws + g.pos[0]), *const starts = (uint32_t*)(ws + g.starts), *const counters = (uint32_t*)(ws + g.counters);
   int row_bits = 0;
   while (rows / kSortBlocks >> row_bits != 0) ++row_bits;
-  const size_t width = (rows / kSortBlocks + 2) & ~1u, smem = kSortWarps * width * 2 + 4 * width;
-  constexpr int kMost = (kSortWarps * 2 + 4) * (kSortRows + 2);
-  static_assert(kMost <= 200 * 1024 && kSortRows == 2 * kSortThreads, "shared memory of the sort, and two rows a thread");
-  static_assert(kSortMost <= 65536, "places fit the counters");
   static std::atomic<uint64_t> ready{0};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return fail(FO_ERR_CUDA, "fo_embed_grad: cannot query the current device");
   if (dev >= 64 || (ready.load() >> dev & 1) == 0) {
-    if (cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost) != cudaSuccess ||
-        cudaFuncSetAttribute(order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost) != cudaSuccess)
+    if (cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortSmem) != cudaSuccess ||
+        cudaFuncSetAttribute(order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortSmem) != cudaSuccess)
       return fail(FO_ERR_CUDA, "fo_embed_grad: cannot set the shared memory size");
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
   bool chained = true;
   cudaError_t e;
-  if (n <= kSortAlone) {
+  if (g.alone) {
     const SortParams p = {f.ids, key, pos, starts, counters, n, rows, n_counters, f.ids_bits, row_bits};
-    e = launch_chained(sort_kernel, kSortBlocks, (unsigned int)kSortThreads, (int)smem, chained, stream, p);
+    e = launch_chained(sort_kernel, kSortBlocks, (unsigned int)kSortThreads, (int)g.sort_smem, chained, stream, p);
   } else {
     const DealParams p = {f.ids, (uint32_t*)(ws + g.key[1]), (uint32_t*)(ws + g.pos[1]), (uint32_t*)(ws + g.hist), key, pos, starts, counters, n, rows,
                           (n + kDealTokens - 1) / kDealTokens, n_counters, f.ids_bits, row_bits};
     e = launch_chained(deal_kernel, p.blocks, (unsigned int)kSortThreads, 0, chained, stream, p);
-    if (e == cudaSuccess) e = launch_chained(order_kernel, kSortBlocks, (unsigned int)kSortThreads, (int)smem, chained, stream, p);
+    if (e == cudaSuccess) e = launch_chained(order_kernel, kSortBlocks, (unsigned int)kSortThreads, (int)g.sort_smem, chained, stream, p);
   }
   return e == cudaSuccess ? FO_OK : fail(FO_ERR_CUDA, "fo_embed_grad: launch failed: %s", cudaGetErrorString(e));
 }
@@ -870,16 +1018,17 @@ extern "C" int fo_embed_grad(const FoEmbedGrad* f, void* cuda_stream) {
     return fail(FO_ERR_INVALID_ARG, "fo_embed_grad: a workspace of %llu bytes, aligned to 16, is needed, got %llu", (unsigned long long)g.bytes, (unsigned long long)f->workspace_bytes);
   cudaStream_t stream = (cudaStream_t)cuda_stream;
   int at = 0;
-  if (int rc = g.several ? sort_in_memory(*f, g, stream, at) : sort_by_rows(*f, g, stream)) return rc;
   char* const ws = (char*)f->workspace;
   p.dy = f->dy; p.out = f->out;
-  p.key = (const uint32_t*)(ws + g.key[at]); p.pos = (const uint32_t*)(ws + g.pos[at]);
   p.starts = (const uint32_t*)(ws + g.starts); p.counters = (uint32_t*)(ws + g.counters);
   p.partial = (float*)(ws + g.partial);
   p.dim = f->dim; p.dy_bytes = (uint32_t)(f->dy_stride * size_of(f->dy_dtype)); p.row_bytes = f->dim * size_of(f->out_dtype);
   p.rows = (uint32_t)f->rows; p.last_token = (uint32_t)(f->n_tokens - 1); p.dealt = !g.several; p.tiles = g.tiles; p.chunk = g.chunk; p.chunks = g.chunks;
   p.factor = (float)(f->scale * factor);
   const bool vectors = f->dim % 8 == 0 && on_16_bytes(f->dy) && f->dy_stride * size_of(f->dy_dtype) % 16 == 0 && on_16_bytes(f->out);
+  if (f->n_tokens <= kFewTokens) return few_tokens(*f, p, vectors, stream);
+  if (int rc = g.several ? sort_in_memory(*f, g, stream, at) : sort_by_rows(*f, g, stream)) return rc;
+  p.key = (const uint32_t*)(ws + g.key[at]); p.pos = (const uint32_t*)(ws + g.pos[at]);
   void (*kernel)(const SumParams) = nullptr;
   int smem = 0;
 #define Y(D, O, V, P, A) \
@@ -898,9 +1047,9 @@ extern "C" int fo_embed_grad(const FoEmbedGrad* f, void* cuda_stream) {
   cudaError_t e = cudaSuccess;
   // (some rings are above the 48 KB that need no word; set at each call: it costs nothing next to the launch)
   if (smem > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (tasks > 0 && e == cudaSuccess) e = launch_chained(kernel, (unsigned int)((tasks + kSumThreads / 32 - 1) / (kSumThreads / 32)), (unsigned int)kSumThreads, smem, chained, stream, p);
+  if (e == cudaSuccess) e = launch_chained(kernel, (unsigned int)((tasks + kSumThreads / 32 - 1) / (kSumThreads / 32)), (unsigned int)kSumThreads, smem, chained, stream, p);
   if (!f->accumulate && e == cudaSuccess) {
-    ClearParams c = {p.starts, (char*)f->out, p.row_bytes, p.rows, 0, p.dealt, tasks == 0};
+    ClearParams c = {p.starts, (char*)f->out, p.row_bytes, p.rows, 0, p.dealt};
     const unsigned long long per_block = (kClearBytes + p.row_bytes - 1) / p.row_bytes;
     c.per_block = (uint32_t)(per_block < kClearThreads / 32 ? kClearThreads / 32 : per_block);
     e = launch_chained(clear_kernel, (p.rows + c.per_block - 1) / c.per_block, (unsigned int)kClearThreads, 0, chained, stream, c);

@@ -266,7 +266,7 @@ def ids_of(kind, n, rows, seed):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("kind", ["uniform", "text", "one", "none", "mixed"])
-@pytest.mark.parametrize("n,rows,dim", [(0, 5, 8), (1, 1, 1), (2, 300, 33), (33, 700, 256), (257, 64, 1001), (1000, 50, 24), (4099, 5000, 264), (9001, 129, 72)])
+@pytest.mark.parametrize("n,rows,dim", [(0, 5, 8), (1, 1, 1), (2, 300, 33), (33, 700, 256), (64, 9000, 5), (65, 40, 520), (257, 64, 1001), (1000, 50, 24), (4099, 5000, 264), (9001, 129, 72)])
 def test_embed_grad_rows(dtype, kind, n, rows, dim):
     import flashoptim_jax_b200 as fo
 

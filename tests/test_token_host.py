@@ -74,7 +74,7 @@ def test_fo_embed_refuses(more, status, text):
     (dict(struct_size=3), 1, b"ABI mismatch"), (dict(dy_dtype=3), 1, b"dy_dtype"), (dict(out_dtype=-1), 1, b"out_dtype"), (dict(ids_bits=0), 1, b"ids_bits"),
     (dict(dropout=_drop(-0.1)), 1, b"p = -0.1"), (dict(out=0), 1, b"null"), (dict(dy=0), 1, b"null"), (dict(dy_stride=7), 1, b"elements apart"),
     (dict(n_tokens=(1 << 31) - 1), 4, b"tokens"), (dict(rows=(1 << 31) - 1), 4, b"rows"), (dict(dim=1 << 24, dy_stride=1 << 24), 4, b"elements"),
-    (dict(workspace_bytes=16), 1, b"workspace"), (dict(workspace=0), 1, b"workspace"), (dict(workspace=72), 1, b"workspace"),
+    (dict(n_tokens=65, workspace_bytes=16), 1, b"workspace"), (dict(n_tokens=65, workspace=0), 1, b"workspace"), (dict(n_tokens=65, workspace=72), 1, b"workspace"),
 ])
 def test_fo_embed_grad_refuses(more, status, text):
     lib = _lib.lib()
@@ -110,8 +110,9 @@ def test_workspace_sizes():
         return out.value
 
     assert need(0, 8, 5) == 0 and need(5, 0, 5) == 0
+    assert need(50257, 768, 1) == 0 and need(50257, 768, 64) == 0  # a handful of tokens needs none
     # keys and positions, and where each row's tokens begin; partial sums of one row at either end of a chunk stay a few megabytes whatever the sizes
-    for rows, dim, n in ((1, 1, 1), (100, 7, 33), (50257, 768, 16384), (128256, 4096, 1 << 20), (2**31 - 2, 8, 2**31 - 2), (8, 2**24 - 1, 4)):
+    for rows, dim, n in ((1, 1, 65), (100, 7, 333), (50257, 768, 16384), (128256, 4096, 1 << 20), (2**31 - 2, 8, 2**31 - 2), (8, 2**24 - 1, 65)):
         assert 8 * n <= need(rows, dim, n) <= 17 * n + 4 * rows + 8 * dim + (64 << 20), (rows, dim, n)
     assert lib.fo_embed_grad_workspace(2**31, 8, 1, ctypes.byref(ctypes.c_uint64())) == 4
     assert lib.fo_embed_grad_workspace(8, 8, 1, None) == 1
