@@ -15,7 +15,7 @@ constexpr int kSms = 148;
 // ---- sizes and the workspace ----------------------------------------------------------------------------------------
 constexpr int kTileCols = 256;     // columns of a warp: eight per lane
 constexpr int kSumThreads = 256, kSumBlocksPerSm = 3;
-constexpr int kLeastChunk = 4;     // tokens
+constexpr int kLeastChunk = 2;     // tokens
 constexpr uint32_t kFewTokens = 64;  // up to so many take one launch and no workspace
 constexpr int kSumWarps = kSms * kSumBlocksPerSm * kSumThreads / 32;  // wanted: all of them resident at once
 
@@ -94,6 +94,32 @@ FO_DEVI void clear_bytes(char* a, char* const b, const int lane) {
   if (a + 2 * lane < up) *(unsigned short*)(a + 2 * lane) = 0;
   for (char* c = up + 16 * lane; c < down; c += 512) *(uint4*)c = make_uint4(0u, 0u, 0u, 0u);
   if (down + 2 * lane < b) *(unsigned short*)(down + 2 * lane) = 0;
+}
+
+// The rows of up to 32 neighbours whose bits are set in `empty`, by one warp: row after row where a row keeps it busy, else in one go over the bytes of all.
+constexpr uint32_t kLongRow = 512;  // bytes
+FO_DEVI void clear_rows(char* const base, const uint32_t rows, const uint32_t empty, const unsigned long long row_bytes, const int lane) {
+  if (row_bytes >= kLongRow) {
+    for (uint32_t left = empty; left != 0; left &= left - 1u) {
+      char* const row = base + (unsigned long long)(__ffs(left) - 1) * row_bytes;
+      clear_bytes(row, row + row_bytes, lane);
+    }
+    return;
+  }
+  if (empty == 0) return;
+  const int size = (int)row_bytes, total = (int)rows * size;
+  for (int at = lane * 16 - (int)((uintptr_t)base & 15); at < total; at += 512) {
+    if (at >= 0 && at + 16 <= total) {
+      const uint32_t r0 = (uint32_t)at / size, r1 = (uint32_t)(at + 15) / size, mask = ((2u << r1) - 1u) & ~((1u << r0) - 1u);
+      if ((empty & mask) == mask) {
+        *(uint4*)(base + at) = make_uint4(0u, 0u, 0u, 0u);
+        continue;
+      }
+      if ((empty & mask) == 0) continue;
+    }
+    for (int b = max(at, 0); b < min(at + 16, total); b += 2)
+      if ((empty >> ((uint32_t)b / size) & 1u) != 0) *(unsigned short*)(base + b) = 0;
+  }
 }
 
 // Exclusive sum over the threads of a block of at most 1024; all of them call it.
@@ -553,20 +579,27 @@ FO_DEVI bool join_pieces(const SumParams& p, const uint32_t chunk, const uint32_
 #pragma unroll 1
   for (int level = 0;; ++level) {
     if (!comes_last(counter, (end - from + step - 1) / step, lane)) return false;
+    float4 t[2] = {};
+#pragma unroll 1
+    for (uint32_t i = from; i < end; i += 4 * step) {
+      float4 a[4][2];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (i + u * step < end) {
+          const float4* const at = (const float4*)piece_at(p, c0 + i + u * step, i + u * step == 0, tile, lane);
+          a[u][0] = __ldcg(at);
+          a[u][1] = __ldcg(at + 1);
+        }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (i + u * step < end) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) t[h] = make_float4(fadd(t[h].x, a[u][h].x), fadd(t[h].y, a[u][h].y), fadd(t[h].z, a[u][h].z), fadd(t[h].w, a[u][h].w));
+        }
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 1
-      for (uint32_t i = from; i < end; i += 4 * step) {
-        float4 a[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (i + u * step < end) a[u] = __ldcg((const float4*)piece_at(p, c0 + i + u * step, i + u * step == 0, tile, lane) + h);
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (i + u * step < end) t = make_float4(fadd(t.x, a[u].x), fadd(t.y, a[u].y), fadd(t.z, a[u].z), fadd(t.w, a[u].w));
-      }
-      sum[4 * h] = t.x; sum[4 * h + 1] = t.y; sum[4 * h + 2] = t.z; sum[4 * h + 3] = t.w;
+      sum[4 * h] = t[h].x; sum[4 * h + 1] = t[h].y; sum[4 * h + 2] = t[h].z; sum[4 * h + 3] = t[h].w;
     }
     if (level == 1 || groups == 1) return true;
     put8(piece_at(p, c0 + g * group, g == 0, tile, lane), sum);
@@ -761,7 +794,15 @@ __global__ void __launch_bounds__(kSumThreads, kSumBlocksPerSm) sum_kernel(const
 
 // Clears the rows without a token, in blocks in the order of the rows: 7.2 TB/s, where a block per SM that walks over its share of them gets 6.2 (128256
 // rows of 8 KB).  Its blocks start beside those of the sums, which are all resident by then, so that one's waiting hides behind the other's writing.
-constexpr int kClearThreads = 256, kClearBytes = 32768;  // of a block, about
+constexpr int kClearThreads = 256, kClearBytes = 32768;
+static_assert(kClearThreads == 8 * 32 && kSumThreads == 8 * 32, "eight warps share 32 rows");
+// Of a block: long rows, one or more a warp, of about 1 / 8 of what an SM has to clear, 4 to 32 KB; or a group of 32 short ones a warp.
+static uint32_t rows_to_clear(const unsigned long long rows, const unsigned long long row_bytes) {
+  unsigned long long bytes = rows * row_bytes / (8 * kSms);
+  bytes = bytes < 4096 ? 4096 : (bytes < kClearBytes ? bytes : kClearBytes);
+  return row_bytes >= kLongRow ? (uint32_t)((bytes / row_bytes + 7) / 8 * 8 + (bytes < row_bytes ? 8 : 0)) : kClearThreads;
+}
+
 struct ClearParams {
   const uint32_t* starts;
   char* out;
@@ -773,12 +814,13 @@ __global__ void __launch_bounds__(kClearThreads) clear_kernel(const __grid_const
   chain_release();  // (no wait: the sums in front have waited for the sort)
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
   const uint32_t r0 = blockIdx.x * p.per_block, r1 = min(r0 + p.per_block, p.rows);
-  for (uint32_t r = r0 + warp; r < r1; r += kClearThreads / 32) {
-    const uint32_t s = p.dealt ? slot_of(r, p.rows) : r;
-    if (p.starts[s] == p.starts[s + 1]) {
-      char* const row = p.out + r * p.row_bytes;
-      clear_bytes(row, row + p.row_bytes, lane);
-    }
+  // 32 rows at a time: the block's warps share them where they are long, else each has its own
+  const bool shared = p.row_bytes >= kLongRow;
+  for (uint32_t r = shared ? r0 : r0 + warp * 32; r < r1; r += shared ? 32 : kClearThreads) {
+    const uint32_t mine = r + lane, s = p.dealt ? slot_of(min(mine, r1 - 1), p.rows) : min(mine, r1 - 1);
+    uint32_t empty = __ballot_sync(~0u, mine < r1 && p.starts[s] == p.starts[s + 1]);
+    if (shared) empty &= 0x01010101u << warp;
+    clear_rows(p.out + r * p.row_bytes, min(32u, r1 - r), empty, p.row_bytes, lane);
   }
   chain_end();
 }
@@ -817,8 +859,13 @@ __global__ void __launch_bounds__(kSumThreads) few_kernel(const __grid_constant_
         if (key[h] >= r0 && key[h] < r1) atomicOr(&named[(key[h] - r0) / 32], 1u << ((key[h] - r0) & 31));
     }
     __syncthreads();
-    for (uint32_t r = r0 + warp; r < r1; r += kSumThreads / 32)
-      if ((named[(r - r0) / 32] >> ((r - r0) & 31) & 1u) == 0) clear_bytes(p.out + r * p.row_bytes, p.out + (r + 1) * p.row_bytes, lane);
+    const bool shared = p.row_bytes >= kLongRow;  // (as in clear_kernel)
+    for (uint32_t r = shared ? r0 : r0 + warp * 32; r < r1; r += shared ? 32 : kSumThreads) {
+      uint32_t empty = ~named[(r - r0) / 32];
+      if (shared) empty &= 0x01010101u << warp;
+      if (r1 - r < 32) empty &= (1u << (r1 - r)) - 1u;
+      clear_rows(p.out + r * p.row_bytes, min(32u, r1 - r), empty, p.row_bytes, lane);
+    }
     return;
   }
   const uint32_t task = blockIdx.x * (kSumThreads / 32) + warp, token = task / p.tiles, tile = task - token * p.tiles;
@@ -902,8 +949,7 @@ static int few_tokens(const FoEmbedGrad& f, const SumParams& s, const bool vecto
   p.token_blocks = (p.n * p.tiles + kSumThreads / 32 - 1) / (kSumThreads / 32);
   unsigned int grid = p.token_blocks;
   if (!f.accumulate) {
-    const unsigned long long per_block = (kClearBytes + s.row_bytes - 1) / s.row_bytes;
-    p.clear_rows = (uint32_t)(per_block < kSumThreads / 32 ? kSumThreads / 32 : per_block);
+    p.clear_rows = rows_to_clear(s.rows, s.row_bytes);
     grid += (p.rows + p.clear_rows - 1) / p.clear_rows;
   }
   if (grid == 0) return FO_OK;
@@ -1050,8 +1096,7 @@ extern "C" int fo_embed_grad(const FoEmbedGrad* f, void* cuda_stream) {
   if (e == cudaSuccess) e = launch_chained(kernel, (unsigned int)((tasks + kSumThreads / 32 - 1) / (kSumThreads / 32)), (unsigned int)kSumThreads, smem, chained, stream, p);
   if (!f->accumulate && e == cudaSuccess) {
     ClearParams c = {p.starts, (char*)f->out, p.row_bytes, p.rows, 0, p.dealt};
-    const unsigned long long per_block = (kClearBytes + p.row_bytes - 1) / p.row_bytes;
-    c.per_block = (uint32_t)(per_block < kClearThreads / 32 ? kClearThreads / 32 : per_block);
+    c.per_block = rows_to_clear(p.rows, p.row_bytes);
     e = launch_chained(clear_kernel, (p.rows + c.per_block - 1) / c.per_block, (unsigned int)kClearThreads, 0, chained, stream, c);
   }
   return e == cudaSuccess ? FO_OK : fail(FO_ERR_CUDA, "fo_embed_grad: launch failed: %s", cudaGetErrorString(e));
