@@ -14,10 +14,12 @@ constexpr int kSms = 148;
 
 // ---- sizes and the workspace ----------------------------------------------------------------------------------------
 constexpr int kTileCols = 256;     // columns of a warp: eight per lane
-constexpr int kSumThreads = 256, kSumBlocksPerSm = 3;
+constexpr int kSumThreads = 256;
+// Resident blocks per SM, and as many warps wanted, all of them resident at once.  With dropout the registers of a third block are worth more to the draws (60000 tokens
+// of 1024 columns 80 us, 86 with three; without it 59 and 56).
+constexpr int sum_blocks_per_sm(const bool drop) { return drop ? 2 : 3; }
 constexpr int kLeastChunk = 2;     // tokens
 constexpr uint32_t kFewTokens = 64;  // up to so many take one launch and no workspace
-constexpr int kSumWarps = kSms * kSumBlocksPerSm * kSumThreads / 32;  // wanted: all of them resident at once
 
 // The sort by rows, in one launch or two: 128 blocks, a 16-bit counter per row and warp.
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
@@ -39,7 +41,8 @@ struct GradPlan {
   unsigned long long key[2], pos[2], starts, counters, hist, total, partial, bytes;  // offsets in the workspace
 };
 
-static GradPlan plan_of(const unsigned long long rows, const unsigned long long dim, const unsigned long long n) {
+// (with dropout there are fewer chunks: the workspace without it has room for them)
+static GradPlan plan_of(const unsigned long long rows, const unsigned long long dim, const unsigned long long n, const bool drop) {
   GradPlan g = {};
   if (n <= kFewTokens) {
     g.tiles = (uint32_t)((dim + kTileCols - 1) / kTileCols);
@@ -50,7 +53,8 @@ static GradPlan plan_of(const unsigned long long rows, const unsigned long long 
   g.alone = !g.several && n <= kSortAlone && (kSortWarps * 2 + 4) * width + lists <= kSortSmem;
   g.sort_smem = g.several ? 0u : (unsigned int)((kSortWarps * 2 + 4) * width + (g.alone ? lists : 0));
   g.tiles = (uint32_t)((dim + kTileCols - 1) / kTileCols);
-  unsigned long long chunk = (n * g.tiles + kSumWarps - 1) / kSumWarps;
+  const unsigned long long warps = kSms * sum_blocks_per_sm(drop) * kSumThreads / 32;
+  unsigned long long chunk = (n * g.tiles + warps - 1) / warps;
   if (chunk < kLeastChunk) chunk = kLeastChunk;
   if (chunk > n) chunk = n;
   g.chunk = (uint32_t)chunk;
@@ -660,7 +664,7 @@ struct Ring {
   static constexpr int kWarp = kStages * kStage, kBlock = kWarp * (kSumThreads / 32);
 };
 template <int DT, int OT, bool VECTORS, bool DROP, bool ACC>
-__global__ void __launch_bounds__(kSumThreads, kSumBlocksPerSm) sum_kernel(const __grid_constant__ SumParams p) {
+__global__ void __launch_bounds__(kSumThreads, sum_blocks_per_sm(DROP)) sum_kernel(const __grid_constant__ SumParams p) {
   chain_wait();
   chain_release();
   using R = Ring<DT, OT, VECTORS, ACC>;
@@ -739,7 +743,7 @@ __global__ void __launch_bounds__(kSumThreads, kSumBlocksPerSm) sum_kernel(const
         const uint32_t at = DROP || !VECTORS ? __shfl_sync(~0u, pos, k) : 0u;
         const unsigned long long e0 = at * p.dim + c0;
         uint4 w = {};
-        if constexpr (DROP && VECTORS) w = draw8(p.drop, off, (e0 >> 3) + lane);
+        if constexpr (DROP && VECTORS) w = draw8(p.drop, off, (unsigned long long)at * (uint32_t)(p.dim / 8) + (tile * (kTileCols / 8) + lane));
         const unsigned char* const stage = group + s * R::kStage;
         if ((heads >> k & 1u) != 0) {  // (the same for the whole warp)
           if (opened) put8(piece_at(p, chunk, false, tile, lane), sum);
@@ -1042,7 +1046,7 @@ extern "C" int fo_embed_grad_workspace(uint64_t rows, uint64_t dim, uint64_t n_t
   if (bytes == nullptr) return fail(FO_ERR_INVALID_ARG, "fo_embed_grad_workspace: null pointer");
   *bytes = 0;
   if (int rc = sizes_ok("fo_embed_grad_workspace", rows, dim, n_tokens)) return rc;
-  if (rows != 0 && dim != 0) *bytes = plan_of(rows, dim, n_tokens).bytes;
+  if (rows != 0 && dim != 0) *bytes = plan_of(rows, dim, n_tokens, false).bytes;
   return FO_OK;
 }
 
@@ -1059,9 +1063,10 @@ extern "C" int fo_embed_grad(const FoEmbedGrad* f, void* cuda_stream) {
   if (f->rows == 0 || f->dim == 0 || (f->accumulate && f->n_tokens == 0)) return FO_OK;
   if (f->out == nullptr || (f->n_tokens > 0 && (f->ids == nullptr || f->dy == nullptr))) return fail(FO_ERR_INVALID_ARG, "fo_embed_grad: null pointer");
   if (f->dy_stride < f->dim || f->dy_stride >> 28) return fail(FO_ERR_INVALID_ARG, "fo_embed_grad: rows %llu elements apart are %llu long", (unsigned long long)f->dy_stride, (unsigned long long)f->dim);
-  const GradPlan g = plan_of(f->rows, f->dim, f->n_tokens);
-  if (f->workspace_bytes < g.bytes || (g.bytes > 0 && (f->workspace == nullptr || !on_16_bytes(f->workspace))))
-    return fail(FO_ERR_INVALID_ARG, "fo_embed_grad: a workspace of %llu bytes, aligned to 16, is needed, got %llu", (unsigned long long)g.bytes, (unsigned long long)f->workspace_bytes);
+  const GradPlan g = plan_of(f->rows, f->dim, f->n_tokens, p.drop.on != 0);
+  const unsigned long long need = plan_of(f->rows, f->dim, f->n_tokens, false).bytes;
+  if (f->workspace_bytes < need || (need > 0 && (f->workspace == nullptr || !on_16_bytes(f->workspace))))
+    return fail(FO_ERR_INVALID_ARG, "fo_embed_grad: a workspace of %llu bytes, aligned to 16, is needed, got %llu", need, (unsigned long long)f->workspace_bytes);
   cudaStream_t stream = (cudaStream_t)cuda_stream;
   int at = 0;
   char* const ws = (char*)f->workspace;
