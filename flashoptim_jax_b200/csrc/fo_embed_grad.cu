@@ -613,30 +613,33 @@ FO_DEVI bool join_pieces(const SumParams& p, const uint32_t chunk, const uint32_
 }
 
 // A tile of a row of DT elements in shared memory.  VECTORS: eight neighbouring elements per lane, which copies and reads its own; otherwise every 32nd, and
-// 16-bit elements come as the words that hold them, with a half in front where the row starts in the middle of a word.
+// the tile comes as the 16 bytes each that hold it, as far into them as it is in memory.
+struct Bounds {  // of the array: nothing outside is touched
+  const char *lo, *hi;
+};
 template <int DT, bool VECTORS>
 struct Tile {
-  static constexpr int kBytes = kTileCols * size_of(DT) + (VECTORS || DT == FO_F32 ? 0 : 16);
-  // `from`: where the tile's first column lies; `count`: columns from the lane's first one on; edge: nothing in front of the tile or behind it may be touched
-  static FO_DEVI void fetch(unsigned char* stage, const char* from, const int columns, const int lane, const bool edge) {
+  static constexpr int kBytes = kTileCols * size_of(DT) + (VECTORS ? 0 : 16);
+  // `from`: where the tile's first column lies
+  static FO_DEVI void fetch(unsigned char* stage, const char* from, const int columns, const int lane, const Bounds in) {
     const uint32_t to = (uint32_t)__cvta_generic_to_shared(stage);
     if constexpr (VECTORS) {
       if (lane * 8 < columns) {
         copy_async16(to + lane * 16, from + lane * 8 * size_of(DT));
         if constexpr (DT == FO_F32) copy_async16(to + 512 + lane * 16, from + lane * 32 + 16);
       }
-    } else if constexpr (DT == FO_F32) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j * 32 + lane < columns) copy_async4(to + (j * 32 + lane) * 4, from + (j * 32 + lane) * 4);
     } else {
-      const int odd = (int)((uintptr_t)from >> 1) & 1;
-      if (edge) {
-        for (int e = lane; e < columns; e += 32) ((unsigned short*)stage)[odd + e] = ((const unsigned short*)from)[e];
+      const int into = (int)((uintptr_t)from & 15), size = (into + columns * size_of(DT) + 15) & ~15;
+      const char* const a = from - into;
+      if (a < in.lo || a + size > in.hi) {
+        for (int e = lane; e < columns; e += 32) {
+          if constexpr (DT == FO_F32) ((uint32_t*)(stage + into))[e] = ((const uint32_t*)from)[e];
+          else ((unsigned short*)(stage + into))[e] = ((const unsigned short*)from)[e];
+        }
       } else {
 #pragma unroll
-        for (int j = 0; j < 5; ++j)
-          if ((j < 4 || lane == 0) && 2 * (j * 32 + lane) - odd < columns) copy_async4(to + (j * 32 + lane) * 4, from - 2 * odd + (j * 32 + lane) * 4);
+        for (int c = 0; c < (kBytes + 511) / 512; ++c)
+          if (c * 512 + lane * 16 < size) copy_async16(to + c * 512 + lane * 16, a + c * 512 + lane * 16);
       }
     }
   }
@@ -647,9 +650,9 @@ struct Tile {
       if constexpr (DT == FO_F32) x.b = *(const uint4*)(stage + 512 + lane * 16);
       x.get(v);
     } else {
-      const int odd = DT == FO_F32 ? 0 : (int)((uintptr_t)from >> 1) & 1;
+      const unsigned char* const at = stage + ((uintptr_t)from & 15);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = load1<DT>(stage, odd + j * 32 + lane);
+      for (int j = 0; j < 8; ++j) v[j] = load1<DT>(at, j * 32 + lane);
     }
   }
 };
@@ -699,14 +702,16 @@ __global__ void __launch_bounds__(kSumThreads, sum_blocks_per_sm(DROP)) sum_kern
     return __ballot_sync(~0u, keys != (lane == 0 ? before : left));
   };
   uint32_t heads = heads_of(key, opened ? row : ~0u), next_key = 0, next_pos = 0, next_heads = 0;
+  const Bounds dy_in = {(const char*)p.dy, (const char*)p.dy + (unsigned long long)p.last_token * p.dy_bytes + p.dim * size_of(DT)};
+  const Bounds out_in = {(const char*)p.out, (const char*)p.out + p.rows * p.row_bytes};
   // token `t` of the 64 at hand into a stage
   auto fetch = [&](const uint32_t t, const uint32_t at, const int stage) {
     unsigned char* const to = ring + stage * R::kStage;
-    Tile<DT, VECTORS>::fetch(to, from + (unsigned long long)at * p.dy_bytes, columns, lane, at == 0 || at == p.last_token);
+    Tile<DT, VECTORS>::fetch(to, from + (unsigned long long)at * p.dy_bytes, columns, lane, dy_in);
     if constexpr (ACC) {
       const uint32_t r = __shfl_sync(~0u, t < 32 ? key : next_key, t & 31);
       if (((t < 32 ? heads : next_heads) >> (t & 31) & 1u) != 0)
-        Tile<OT, VECTORS>::fetch(to + R::kOld, out + r * p.row_bytes, columns, lane, r == 0 || r == p.rows - 1);
+        Tile<OT, VECTORS>::fetch(to + R::kOld, out + r * p.row_bytes, columns, lane, out_in);
     }
   };
 #pragma unroll
