@@ -204,9 +204,10 @@ def host():
         from .quantization import QuantizedArray
 
         names = ("fo_step_ex", "fo_sq_norm_mixed", "fo_split_many", "fo_reconstruct_many", "fo_quantize_momentum", "fo_quantize_variance",
-                 "fo_dequantize_momentum", "fo_dequantize_variance", "fo_dropout", "fo_embed", "fo_embed_grad", "fo_embed_grad_workspace",
-                 "fo_status_string", "fo_last_error")
+                 "fo_dequantize_momentum", "fo_dequantize_variance", "fo_status_string", "fo_last_error")
+        tokens = ("fo_dropout", "fo_embed", "fo_embed_grad", "fo_embed_grad_workspace")
         _fo_host.bind({name: ctypes.cast(getattr(l, name), ctypes.c_void_p).value for name in names}, QuantizedArray)
+        _fo_host.bind_tokens({name: ctypes.cast(getattr(l, name), ctypes.c_void_p).value for name in tokens})
         _host = _fo_host
     return _host
 

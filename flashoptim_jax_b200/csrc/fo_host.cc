@@ -1200,20 +1200,30 @@ PyObject* embed_grad(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   return a[7];
 }
 
+template <typename F>
+bool address(PyObject* d, const char* name, F& fn) {
+  PyObject* v = PyDict_GetItemString(d, name);
+  if (v == nullptr) { PyErr_Format(PyExc_KeyError, "%s", name); return false; }
+  fn = reinterpret_cast<F>(PyLong_AsVoidPtr(v));
+  return PyErr_Occurred() == nullptr;
+}
+// bind_tokens({name: address})
+PyObject* bind_tokens(PyObject*, PyObject* args) {
+  PyObject* d;
+  if (!PyArg_ParseTuple(args, "O!", &PyDict_Type, &d)) return nullptr;
+  if (!address(d, "fo_dropout", api.dropout) || !address(d, "fo_embed", api.embed) || !address(d, "fo_embed_grad", api.embed_grad) ||
+      !address(d, "fo_embed_grad_workspace", api.embed_grad_workspace))
+    return nullptr;
+  Py_RETURN_NONE;
+}
 // bind({name: address}, QuantizedArray)
 PyObject* bind(PyObject*, PyObject* args) {
   PyObject *d, *type;
   if (!PyArg_ParseTuple(args, "O!O", &PyDict_Type, &d, &type)) return nullptr;
-  auto get = [&](const char* name, auto& fn) {
-    PyObject* v = PyDict_GetItemString(d, name);
-    if (v == nullptr) { PyErr_Format(PyExc_KeyError, "%s", name); return false; }
-    fn = reinterpret_cast<std::remove_reference_t<decltype(fn)>>(PyLong_AsVoidPtr(v));
-    return PyErr_Occurred() == nullptr;
-  };
+  auto get = [&](const char* name, auto& fn) { return address(d, name, fn); };
   if (!get("fo_step_ex", api.step) || !get("fo_sq_norm_mixed", api.sq_norm) || !get("fo_split_many", api.split) || !get("fo_reconstruct_many", api.reconstruct) ||
       !get("fo_quantize_momentum", api.quantize_m) || !get("fo_quantize_variance", api.quantize_v) || !get("fo_dequantize_momentum", api.dequantize_m) ||
-      !get("fo_dequantize_variance", api.dequantize_v) || !get("fo_dropout", api.dropout) || !get("fo_embed", api.embed) ||
-      !get("fo_embed_grad", api.embed_grad) || !get("fo_embed_grad_workspace", api.embed_grad_workspace) || !get("fo_status_string", api.status_string) || !get("fo_last_error", api.last_error))
+      !get("fo_dequantize_variance", api.dequantize_v) || !get("fo_status_string", api.status_string) || !get("fo_last_error", api.last_error))
     return nullptr;
   Ref collections(PyImport_ImportModule("collections"));
   Ref ordered(collections.p == nullptr ? nullptr : PyObject_GetAttrString(collections.p, "OrderedDict"));
@@ -1246,6 +1256,7 @@ PyObject* guarded_args(PyObject* self, PyObject* args) {
 
 PyMethodDef methods[] = {
     {"bind", (PyCFunction)(void*)guarded_args<bind>, METH_VARARGS, nullptr},
+    {"bind_tokens", (PyCFunction)(void*)guarded_args<bind_tokens>, METH_VARARGS, nullptr},
     {"make_plan", (PyCFunction)(void*)guarded_args<make_plan>, METH_VARARGS, nullptr},
     {"run", (PyCFunction)(void*)guarded<run>, METH_FASTCALL, nullptr},
     {"sq_norm", (PyCFunction)(void*)guarded<sq_norm>, METH_FASTCALL, nullptr},

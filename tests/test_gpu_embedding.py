@@ -302,6 +302,47 @@ def test_embed_grad_of_many_tokens(kind, n, rows, dim):
     check_grad(fo.embed_grad(dy, ids, rows, out=before.clone(), accumulate=True, p=0.25, seed=2), dy, ids, rows, torch.float32, p=0.25, seed=2, before=before)
 
 
+@pytest.mark.parametrize("n,rows,dim", [(8192, 262_143, 8), (8193, 262_143, 8), (100, 262_144, 8), (8193, 262_144, 8), (30_000, 3, 300), (5000, 127, 16), (5000, 129, 16),
+                                        (20_000, 1, 520), (65, 70_000, 3), (2048, 2048, 2048)])
+def test_embed_grad_where_the_ways_to_sort_meet(n, rows, dim):
+    import flashoptim_jax_b200 as fo
+
+    for kind in ("uniform", "text", "mixed"):
+        ids, dy = ids_of(kind, n, rows, 7), rand((n, dim), torch.float16, 8)
+        got = fo.embed_grad(dy, ids, rows, scale=0.5)
+        check_grad(got, dy, ids, rows, torch.float16, scale=0.5)
+        assert torch.equal(got, fo.embed_grad(dy, ids, rows, scale=0.5))
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_random_sizes(seed):
+    """Sizes spread over three orders of magnitude, odd and even widths, every type, dropout, views into larger buffers."""
+    import random
+
+    import flashoptim_jax_b200 as fo
+
+    rng = random.Random(seed)
+
+    def log(lo, hi):
+        return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+    dt = rng.choice(list(DTYPES.values()))
+    dim = rng.choice([8 * log(1, 100), log(1, 900)])
+    rows, n = log(1, 20_000), log(1, min(30_000, 6_000_000 // dim))
+    p, scale, offset = rng.choice([0.0, 0.1, 0.77]), rng.choice([1.0, -3.7]), rng.randrange(2**40)
+    pad = rng.choice([0, 0, 1, 5])
+    ids = ids_of(rng.choice(["uniform", "text", "mixed"]), n, rows, seed)
+    dy = rand((n, dim + pad), dt, seed)[:, pad // 2:pad // 2 + dim]
+    check_grad(fo.embed_grad(dy, ids, rows, scale=scale, p=p, seed=seed, offset=offset), dy, ids, rows, dt, scale, p, seed, offset)
+    before = rand((rows, dim), torch.float32, seed + 1)
+    got = fo.embed_grad(dy, ids, rows, scale=scale, p=p, seed=seed, offset=offset, out=before.clone(), accumulate=True)
+    check_grad(got, dy, ids, rows, torch.float32, scale, p, seed, offset, before=before)
+    table = rand((rows, dim + pad), dt, seed + 2)[:, pad // 2:pad // 2 + dim]
+    y = fo.embed(table, ids, scale=scale, p=p, seed=seed, offset=offset)
+    element_close(y, T.embed(f64(table), ids.cpu().numpy(), scale, p, seed, offset), dt)
+    element_close(fo.dropout(dy, p, seed, offset), T.dropout(f64(dy), p, seed, offset), dt)
+
+
 @pytest.mark.parametrize("n", [5, 3000, 80_000])
 def test_untouched_rows_keep_their_bits(n):
     import flashoptim_jax_b200 as fo
@@ -474,6 +515,41 @@ def test_calls_on_two_streams_do_not_meet():
         assert torch.equal(g, want[k % len(cases)])
 
 
+def test_two_threads_at_once():
+    import threading
+
+    import flashoptim_jax_b200 as fo
+
+    cases = [(rand((n, 264), torch.float32, n), ids_of("mixed", n, 900, n)) for n in (40, 3000, 20_000)]
+
+    def work(dy, ids):
+        y = fo.dropout(dy, 0.2, 1, 2)
+        g = fo.embed_grad(y, ids, 900)
+        return g, fo.embed(g, ids.clamp(max=899), p=0.1, seed=3)
+
+    want = [work(*c) for c in cases]
+    torch.cuda.synchronize()
+    got, errors = {}, []
+
+    def run(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[k] = work(*cases[k])
+            torch.cuda.synchronize()
+        except Exception as e:  # noqa: BLE001 (reported below)
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(k,)) for k in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for k, w in enumerate(want):
+        assert all(torch.equal(x, y) for x, y in zip(got[k], w))
+
+
 def test_dependent_calls_see_each_other():
     """Each call's input is what the one in front of it has just written, without a wait between them."""
     import flashoptim_jax_b200 as fo
@@ -535,6 +611,27 @@ def test_a_step_on_token_gradients(name, how):
     assert len(a) == len(b)
     for x, y in zip(a, b):
         assert torch.equal(x, y)
+
+
+def test_a_sharded_step_on_token_gradients():
+    """Zero1Optimizer on one rank: a TokenGradient goes straight into the flat gradient buffer."""
+    import flashoptim_jax_b200 as fo
+    from flashoptim_jax_b200 import tree as pytree
+    from flashoptim_jax_b200.zero1 import Zero1Optimizer
+
+    def params():
+        return {"a": torch.ones(33, device="cuda"), "wte": rand((500, 70), torch.bfloat16, 1, std=0.02), "z": rand((11, 7), torch.bfloat16, 2)}
+
+    one, two = (Zero1Optimizer("adamw", params(), learning_rate=1e-3, weight_decay=1e-2, master_weight_bits=32) for _ in range(2))
+    for k in range(3):
+        ids, dy = ids_of("mixed", 700, 500, k), rand((700, 70), torch.bfloat16, k)
+        rest = {"a": rand((33,), torch.float32, k), "z": rand((11, 7), torch.bfloat16, k)}
+        one.step({**rest, "wte": fo.TokenGradient(dy, ids, scale=2.0)})
+        two.step({**rest, "wte": fo.embed_grad(dy, ids, 500, scale=2.0)})
+    for x, y in zip(pytree.tree_leaves(one.params), pytree.tree_leaves(two.params)):
+        assert torch.equal(x, y)
+    with pytest.raises(TypeError, match="narrowed"):  # as for any other gradient
+        one.step({**rest, "wte": fo.TokenGradient(dy.float(), ids)})
 
 
 def test_a_token_gradient_for_the_wrong_leaf_is_refused():
