@@ -359,22 +359,34 @@ __global__ void __launch_bounds__(kSortThreads) order_kernel(const __grid_consta
   const uint32_t tokens = pile_begin[p.blocks], before = smaller;
   const uint32_t rounds = (tokens + kSortThreads - 1) / kSortThreads, warps = rounds == 0 ? 0u : (tokens + rounds * 32 - 1) / (rounds * 32);
   unsigned short* const my_counts = counts + warp * width;
-  auto walk = [&](auto f) {
-    if (warp >= (int)warps) return;
-#pragma unroll 1
-    for (uint32_t r = 0; r < rounds; ++r) {
-      const uint32_t t = (warp * rounds + r) * 32 + lane;
-      uint32_t pile = 0;
-      for (uint32_t step = kDealBlocksMost / 2; step != 0; step /= 2)
-        if (pile + step < p.blocks && pile_begin[pile + step] <= t) pile += step;
-      const bool in = t < tokens;
-      const uint32_t from = pile_at[pile] + t - pile_begin[pile];
-      const uint32_t key = in ? p.pile_key[from] : 0u;
-      const uint32_t rank = rank_in_warp(key / kSortBlocks, in, p.row_bits, my_counts, lane);
-      if (in) f(key, rank, from);
-    }
+  // a token of this block's: where it lies in the piles, its key and its rank among the warp's tokens of its row
+  struct Found {
+    bool in;
+    uint32_t key, rank, from;
   };
-  walk([](uint32_t, uint32_t, uint32_t) {});
+  auto find = [&](const uint32_t r) {
+    Found t;
+    const uint32_t i = (warp * rounds + r) * 32 + lane;
+    uint32_t pile = 0;
+    for (uint32_t step = kDealBlocksMost / 2; step != 0; step /= 2)
+      if (pile + step < p.blocks && pile_begin[pile + step] <= i) pile += step;
+    t.in = i < tokens;
+    t.from = pile_at[pile] + i - pile_begin[pile];
+    t.key = t.in ? p.pile_key[t.from] : 0u;
+    t.rank = rank_in_warp(t.key / kSortBlocks, t.in, p.row_bits, my_counts, lane);
+    return t;
+  };
+  Found only = {};  // of one round, which is the usual case, nothing is looked up again
+  uint32_t only_pos = 0;
+  if (warp < (int)warps) {
+    if (rounds == 1) {
+      only = find(0);
+      if (only.in) only_pos = p.pile_pos[only.from];
+    } else {
+#pragma unroll 1
+      for (uint32_t r = 0; r < rounds; ++r) find(r);
+    }
+  }
   __syncthreads();
   uint32_t total[2] = {0u, 0u}, all;
 #pragma unroll
@@ -397,11 +409,21 @@ __global__ void __launch_bounds__(kSortThreads) order_kernel(const __grid_consta
   }
   if (me == kSortBlocks - 1 && threadIdx.x == 0) p.starts[p.rows] = before + all;
   __syncthreads();
-  walk([&](const uint32_t key, const uint32_t rank, const uint32_t from) {
-    const uint32_t to = first[key / kSortBlocks] + rank;
+  auto put = [&](const uint32_t to, const uint32_t key, const uint32_t pos) {
     p.key_out[to] = key;
-    p.pos_out[to] = p.pile_pos[from];
-  });
+    p.pos_out[to] = pos;
+  };
+  if (warp < (int)warps) {
+    if (rounds == 1) {
+      if (only.in) put(first[only.key / kSortBlocks] + my_counts[only.key / kSortBlocks] + only.rank, only.key, only_pos);
+    } else {  // the counters now say where the warp's tokens begin: counting on gives each its place
+#pragma unroll 1
+      for (uint32_t r = 0; r < rounds; ++r) {
+        const Found t = find(r);
+        if (t.in) put(first[t.key / kSortBlocks] + t.rank, t.key, p.pile_pos[t.from]);
+      }
+    }
+  }
 }
 
 // More tokens, or more rows: least digit first, three launches per digit.
@@ -556,33 +578,36 @@ FO_DEVI void put8(float* to, const float (&v)[8]) {
   __stcg((float4*)to, make_float4(v[0], v[1], v[2], v[3]));
   __stcg((float4*)to + 1, make_float4(v[4], v[5], v[6], v[7]));
 }
-// true for all lanes of the warp that comes last of `of`
-FO_DEVI bool comes_last(uint32_t* counter, const uint32_t of, const int lane) {
-  __threadfence();
-  __syncwarp();
-  uint32_t seen = 0;
-  if (lane == 0) seen = atomicAdd(counter, 1u);
-  const bool last = __shfl_sync(~0u, seen, 0) + 1 == of;
-  if (last) __threadfence();
-  return last;
-}
-
 // Where the partial sum of a chunk's first row (begun in an earlier chunk) or last row (going on in the next) lies.
 FO_DEVI float* piece_at(const SumParams& p, const uint32_t chunk, const bool last, const uint32_t tile, const int lane) {
   return p.partial + (((unsigned long long)chunk * 2 + (last ? 1 : 0)) * p.tiles + tile) * kTileCols + lane * 8;
 }
-// `chunk` has left its piece of a row whose tokens lie in the chunks c0 ... c1; true: it is the last to come, and the row's sum is in `sum`.  The pieces are
-// added up in groups of about the square root of their number, the groups by the last of them to come, in the order of the tokens whoever comes
-// last: the sum does not depend on it.  (One warp adding up 500 pieces would take longer than everything else.)
-FO_DEVI bool join_pieces(const SumParams& p, const uint32_t chunk, const uint32_t c0, const uint32_t c1, const uint32_t tile, const int lane, float (&sum)[8]) {
-  const uint32_t pieces = c1 - c0 + 1, group = max(16u, (uint32_t)ceilf(sqrtf((float)pieces)));
-  const uint32_t g = (chunk - c0) / group, groups = (pieces + group - 1) / group, cells = p.chunks * p.tiles;
+// The pieces of a row whose tokens lie in the chunks c0 ... c1, as `chunk`, one of them, sees them.  They are added up in groups of about the square root of their
+// number by the last of each to come, the groups by the last of those, in the order of the tokens whoever comes last: the sum does not depend on
+// it.  (One warp adding up 500 pieces would take longer than everything else.)
+struct Pieces {
+  uint32_t c0, pieces, group, groups, from, end;  // from ... end - 1: the chunk's group
+  uint32_t* counter;                              // of the group
+};
+FO_DEVI Pieces pieces_of(const SumParams& p, const uint32_t chunk, const uint32_t c0, const uint32_t c1, const uint32_t tile) {
+  Pieces r;
+  r.c0 = c0;
+  r.pieces = c1 - c0 + 1;
+  r.group = max(16u, (uint32_t)ceilf(sqrtf((float)r.pieces)));
+  const uint32_t g = (chunk - c0) / r.group;
+  r.groups = (r.pieces + r.group - 1) / r.group;
+  r.from = g * r.group;
+  r.end = min(r.from + r.group, r.pieces);
   // (a chunk may hold the first piece of one row and begin a group of another: they count apart)
-  uint32_t* counter = p.counters + (g == 0 ? 0u : cells) + (c0 + g * group) * p.tiles + tile;
-  uint32_t from = g * group, end = min(from + group, pieces), step = 1;
+  r.counter = p.counters + (g == 0 ? 0u : p.chunks * p.tiles) + (c0 + r.from) * p.tiles + tile;
+  return r;
+}
+// The whole sum of a row in `sum` (true), once all pieces of the chunk's group are there, if that was the last group.
+FO_DEVI bool join_pieces(const SumParams& p, const Pieces& r, const uint32_t tile, const int lane, float (&sum)[8]) {
+  uint32_t from = r.from, end = r.end, step = 1;
 #pragma unroll 1
   for (int level = 0;; ++level) {
-    if (!comes_last(counter, (end - from + step - 1) / step, lane)) return false;
+    __threadfence();
     float4 t[2] = {};
 #pragma unroll 1
     for (uint32_t i = from; i < end; i += 4 * step) {
@@ -590,7 +615,7 @@ FO_DEVI bool join_pieces(const SumParams& p, const uint32_t chunk, const uint32_
 #pragma unroll
       for (int u = 0; u < 4; ++u)
         if (i + u * step < end) {
-          const float4* const at = (const float4*)piece_at(p, c0 + i + u * step, i + u * step == 0, tile, lane);
+          const float4* const at = (const float4*)piece_at(p, r.c0 + i + u * step, i + u * step == 0, tile, lane);
           a[u][0] = __ldcg(at);
           a[u][1] = __ldcg(at + 1);
         }
@@ -605,10 +630,14 @@ FO_DEVI bool join_pieces(const SumParams& p, const uint32_t chunk, const uint32_
     for (int h = 0; h < 2; ++h) {
       sum[4 * h] = t[h].x; sum[4 * h + 1] = t[h].y; sum[4 * h + 2] = t[h].z; sum[4 * h + 3] = t[h].w;
     }
-    if (level == 1 || groups == 1) return true;
-    put8(piece_at(p, c0 + g * group, g == 0, tile, lane), sum);
-    counter = p.counters + 2 * cells + c0 * p.tiles + tile;
-    from = 0; end = pieces; step = group;
+    if (level == 1 || r.groups == 1) return true;
+    put8(piece_at(p, r.c0 + from, from == 0, tile, lane), sum);
+    __threadfence();
+    __syncwarp();
+    uint32_t seen = 0;
+    if (lane == 0) seen = atomicAdd(p.counters + 2 * p.chunks * p.tiles + r.c0 * p.tiles + tile, 1u);
+    if (__shfl_sync(~0u, seen, 0) + 1 != r.groups) return false;
+    from = 0; end = r.pieces; step = r.group;
   }
 }
 
@@ -792,12 +821,22 @@ __global__ void __launch_bounds__(kSumThreads, sum_blocks_per_sm(DROP)) sum_kern
   if (opened) put8(piece_at(p, chunk, false, tile, lane), sum);
   else if (goes_on) put8(piece_at(p, chunk, true, tile, lane), sum);
   else write_row<OT, VECTORS>(out + row * p.row_bytes + lane * kLaneOut, count, sum);
-  // the pieces: of the row that began earlier, then of the one that goes on
+  // The pieces: of the row that began earlier (lane 0 counts), and of the one that goes on (lane 1).
+  const bool first_left = row_begins < first, last_left = !opened && goes_on;
+  if (!first_left && !last_left) return;
+  __threadfence();
+  __syncwarp();
+  bool came_last = false;
+  if (lane == 0 ? first_left : lane == 1 && last_left) {
+    const Pieces r = pieces_of(p, chunk, lane == 0 ? row_begins / p.chunk : chunk, ((lane == 0 ? row_ends : last_ends) - 1) / p.chunk, tile);
+    came_last = atomicAdd(r.counter, 1u) + 1 == r.end - r.from;
+  }
+  const uint32_t to_join = __ballot_sync(~0u, came_last);
 #pragma unroll 1
   for (int which = 0; which < 2; ++which) {
-    if (which == 0 ? row_begins >= first : opened || !goes_on) continue;
-    const uint32_t c0 = which == 0 ? row_begins / p.chunk : chunk, c1 = ((which == 0 ? row_ends : last_ends) - 1) / p.chunk;
-    if (join_pieces(p, chunk, c0, c1, tile, lane, sum)) write_row<OT, VECTORS>(out + (which == 0 ? first_row : last_row) * p.row_bytes + lane * kLaneOut, count, sum);
+    if ((to_join >> which & 1u) == 0) continue;
+    const Pieces r = pieces_of(p, chunk, which == 0 ? row_begins / p.chunk : chunk, ((which == 0 ? row_ends : last_ends) - 1) / p.chunk, tile);
+    if (join_pieces(p, r, tile, lane, sum)) write_row<OT, VECTORS>(out + (which == 0 ? first_row : last_row) * p.row_bytes + lane * kLaneOut, count, sum);
   }
 }
 
