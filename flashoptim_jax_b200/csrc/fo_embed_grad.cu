@@ -367,33 +367,38 @@ __global__ void __launch_bounds__(kSortThreads) order_kernel(const __grid_consta
   const uint32_t tokens = pile_begin[p.blocks], before = smaller;
   const uint32_t rounds = (tokens + kSortThreads - 1) / kSortThreads, warps = rounds == 0 ? 0u : (tokens + rounds * 32 - 1) / (rounds * 32);
   unsigned short* const my_counts = counts + warp * width;
-  // a token of this block's: where it lies in the piles, its key and its rank among the warp's tokens of its row
-  struct Found {
-    bool in;
-    uint32_t key, rank, from;
-  };
-  auto find = [&](const uint32_t r) {
-    Found t;
-    const uint32_t i = (warp * rounds + r) * 32 + lane;
-    uint32_t pile = 0;
+  // f(key, rank among the warp's tokens of its row, position) for this block's tokens, four rounds' loads at once
+  auto walk = [&](auto with_pos, auto f) {
+    uint32_t pile = 0;  // the one that holds the lane's next token: sought once, then followed
     for (uint32_t step = kDealBlocksMost / 2; step != 0; step /= 2)
-      if (pile + step < p.blocks && pile_begin[pile + step] <= i) pile += step;
-    t.in = i < tokens;
-    t.from = pile_at[pile] + i - pile_begin[pile];
-    t.key = t.in ? p.pile_key[t.from] : 0u;
-    t.rank = rank_in_warp(t.key / kSortBlocks, t.in, p.row_bits, my_counts, lane);
-    return t;
-  };
-  Found only = {};  // of one round, which is the usual case, nothing is looked up again
-  uint32_t only_pos = 0;
-  if (warp < (int)warps) {
-    if (rounds == 1) {
-      only = find(0);
-      if (only.in) only_pos = p.pile_pos[only.from];
-    } else {
+      if (pile + step < p.blocks && pile_begin[pile + step] <= warp * rounds * 32 + lane) pile += step;
 #pragma unroll 1
-      for (uint32_t r = 0; r < rounds; ++r) find(r);
+    for (uint32_t r0 = 0; r0 < rounds; r0 += 4) {
+      uint32_t key[4], pos[4];
+      bool in[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t i = (warp * rounds + r0 + r) * 32 + lane;
+        in[r] = r0 + r < rounds && i < tokens;
+        while (pile + 1 < p.blocks && pile_begin[pile + 1] <= i) ++pile;
+        const uint32_t from = pile_at[pile] + i - pile_begin[pile];
+        key[r] = in[r] ? p.pile_key[from] : 0u;
+        pos[r] = decltype(with_pos)::value && in[r] ? p.pile_pos[from] : 0u;
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (r0 + r >= rounds) break;
+        const uint32_t rank = rank_in_warp(key[r] / kSortBlocks, in[r], p.row_bits, my_counts, lane);
+        if (in[r]) f(key[r], rank, pos[r]);
+      }
     }
+  };
+  uint32_t only_key = 0, only_rank = ~0u, only_pos = 0;  // of one round, which is the usual case, nothing is looked up again
+  if (warp < (int)warps) {
+    if (rounds == 1)
+      walk(std::true_type{}, [&](const uint32_t key, const uint32_t rank, const uint32_t pos) { only_key = key, only_rank = rank, only_pos = pos; });
+    else
+      walk(std::false_type{}, [](uint32_t, uint32_t, uint32_t) {});
   }
   __syncthreads();
   uint32_t total[2] = {0u, 0u}, all;
@@ -423,13 +428,9 @@ __global__ void __launch_bounds__(kSortThreads) order_kernel(const __grid_consta
   };
   if (warp < (int)warps) {
     if (rounds == 1) {
-      if (only.in) put(first[only.key / kSortBlocks] + my_counts[only.key / kSortBlocks] + only.rank, only.key, only_pos);
+      if (only_rank != ~0u) put(first[only_key / kSortBlocks] + my_counts[only_key / kSortBlocks] + only_rank, only_key, only_pos);
     } else {  // the counters now say where the warp's tokens begin: counting on gives each its place
-#pragma unroll 1
-      for (uint32_t r = 0; r < rounds; ++r) {
-        const Found t = find(r);
-        if (t.in) put(first[t.key / kSortBlocks] + t.rank, t.key, p.pile_pos[t.from]);
-      }
+      walk(std::true_type{}, [&](const uint32_t key, const uint32_t rank, const uint32_t pos) { put(first[key / kSortBlocks] + rank, key, pos); });
     }
   }
 }
@@ -437,8 +438,8 @@ __global__ void __launch_bounds__(kSortThreads) order_kernel(const __grid_consta
 // More tokens, or more rows: least digit first, three launches per digit.
 struct RadixParams {
   const void* ids;
-  const uint32_t* key_in;  // null: the ids
-  const uint32_t* pos_in;
+  uint32_t* key_in;        // of the first digit, written by the counting from the ids, which are read once: the passes agree whatever another stream does to them
+  const uint32_t* pos_in;  // null: the tokens in their order
   uint32_t* key_out;
   uint32_t* pos_out;
   uint32_t* hist;   // [bin][block]
@@ -446,8 +447,6 @@ struct RadixParams {
   uint32_t n, rows, blocks;
   int32_t ids_bits, shift, digit_bits;
 };
-FO_DEVI uint32_t radix_key(const RadixParams& p, const uint32_t i) { return p.key_in != nullptr ? p.key_in[i] : key_of(id_at(p.ids, p.ids_bits, i), p.rows); }
-
 __global__ void __launch_bounds__(kRadixThreads) radix_count_kernel(const __grid_constant__ RadixParams p) {
   chain_wait();
   chain_release();
@@ -458,7 +457,11 @@ __global__ void __launch_bounds__(kRadixThreads) radix_count_kernel(const __grid
 #pragma unroll
   for (int r = 0; r < kRadixRounds; ++r) {
     const unsigned long long i = (unsigned long long)blockIdx.x * kRadixTile + r * kRadixThreads + threadIdx.x;
-    if (i < p.n) atomicAdd(&count[(radix_key(p, (uint32_t)i) >> p.shift) & mask], 1u);
+    if (i < p.n) {
+      const uint32_t key = p.shift == 0 ? key_of(id_at(p.ids, p.ids_bits, i), p.rows) : p.key_in[i];
+      if (p.shift == 0) p.key_in[i] = key;
+      atomicAdd(&count[(key >> p.shift) & mask], 1u);
+    }
   }
   __syncthreads();
   for (int i = threadIdx.x; i < kBinsMax; i += kRadixThreads) p.hist[(unsigned long long)i * p.blocks + blockIdx.x] = count[i];
@@ -507,7 +510,7 @@ __global__ void __launch_bounds__(kRadixThreads) radix_scatter_kernel(const __gr
   const unsigned long long i0 = (unsigned long long)blockIdx.x * kRadixTile + warp * (kRadixRounds * 32) + lane;
   uint32_t key[kRadixRounds], rank[kRadixRounds];
 #pragma unroll
-  for (int r = 0; r < kRadixRounds; ++r) key[r] = i0 + r * 32 < p.n ? radix_key(p, (uint32_t)(i0 + r * 32)) : 0u;
+  for (int r = 0; r < kRadixRounds; ++r) key[r] = i0 + r * 32 < p.n ? p.key_in[i0 + r * 32] : 0u;
 #pragma unroll
   for (int r = 0; r < kRadixRounds; ++r) rank[r] = rank_in_warp((key[r] >> p.shift) & mask, i0 + r * 32 < p.n, p.digit_bits, counts[warp], lane);
   __syncthreads();
@@ -526,7 +529,6 @@ __global__ void __launch_bounds__(kRadixThreads) radix_scatter_kernel(const __gr
   for (int r = 0; r < kRadixRounds; ++r) {
     if (i0 + r * 32 < p.n) {
       const uint32_t digit = (key[r] >> p.shift) & mask, to = base[digit] + counts[warp][digit] + rank[r];
-      if (to >= p.n) continue;  // (ids that another stream changed meanwhile)
       p.key_out[to] = key[r];
       p.pos_out[to] = p.pos_in != nullptr ? p.pos_in[i0 + r * 32] : (uint32_t)(i0 + r * 32);
     }
@@ -1073,7 +1075,7 @@ static int sort_in_memory(const FoEmbedGrad& f, const GradPlan& g, cudaStream_t 
   p.n = (uint32_t)f.n_tokens; p.rows = (uint32_t)f.rows; p.blocks = g.blocks;
   cudaError_t e = cudaSuccess;
   for (int pass = 0; pass < passes && e == cudaSuccess; ++pass) {
-    p.key_in = pass == 0 ? nullptr : (const uint32_t*)(ws + g.key[(pass - 1) & 1]);
+    p.key_in = (uint32_t*)(ws + g.key[(pass + 1) & 1]);
     p.pos_in = pass == 0 ? nullptr : (const uint32_t*)(ws + g.pos[(pass - 1) & 1]);
     p.key_out = (uint32_t*)(ws + g.key[pass & 1]); p.pos_out = (uint32_t*)(ws + g.pos[pass & 1]);
     p.shift = pass * p.digit_bits;
