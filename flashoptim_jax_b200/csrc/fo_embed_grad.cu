@@ -36,7 +36,8 @@ constexpr unsigned long long kSortAlone = 8192;  // of which up to so many take 
 constexpr int kSortSmem = 220 * 1024;
 static_assert(kSortRows == 2 * kSortThreads && (kSortWarps * 2 + 4) * (kSortRows + 2) <= kSortSmem && kSortMost <= 65536, "two rows a thread, shared memory, places that fit the counters");
 // More than 65536 tokens (a place no longer fits 16 bits) or 262143 rows (nor do the counters the shared memory): the sort by digits, three launches for each
-// digit of at most nine bits, tiles of 4096 tokens.
+// digit of at most nine bits, tiles of 4096 tokens.  It takes as long whatever the ids are: 131072 tokens of 768 columns into 50257 rows 89 us, where the sort by rows with counters
+// of 32 bits took 76, but 130 with 0.4 of the tokens of one id, which are all one block's.
 constexpr int kDigitMax = 9, kBinsMax = 1 << kDigitMax;
 constexpr int kRadixThreads = 512, kRadixRounds = 8, kRadixTile = kRadixThreads * kRadixRounds;
 

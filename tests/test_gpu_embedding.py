@@ -303,7 +303,7 @@ def test_embed_grad_of_many_tokens(kind, n, rows, dim):
 
 
 @pytest.mark.parametrize("n,rows,dim", [(8192, 262_143, 8), (8193, 262_143, 8), (100, 262_144, 8), (8193, 262_144, 8), (30_000, 3, 300), (5000, 127, 16), (5000, 129, 16),
-                                        (20_000, 1, 520), (65, 70_000, 3), (2048, 2048, 2048)])
+                                        (20_000, 1, 520), (65, 70_000, 3), (2048, 2048, 2048), (65_537, 212_991, 8), (65_537, 212_992, 8), (1_048_577, 500, 8)])
 def test_embed_grad_where_the_ways_to_sort_meet(n, rows, dim):
     import flashoptim_jax_b200 as fo
 
