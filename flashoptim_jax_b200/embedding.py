@@ -89,7 +89,8 @@ def embed(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, ecc: Op
     are the fp32 weights that `reconstruct_leaf` gives; the 0-d marker of a leaf without codes is taken for none.  The result has the table's dtype, with
     `ecc` fp32; `dtype` may ask for either.  `ids`: int32 or int64.  A negative id is no token: its row is 0 and it has no part in the
     gradient.  An id behind the last row cannot be reported without waiting for the GPU: its row is NaN, which the loss shows.
-    Differentiable in the table (once): the gradient is `embed_grad`'s, in the table's dtype."""
+    Differentiable in the table (once): the gradient is `embed_grad`'s, in the table's dtype.  A step that is captured in a CUDA graph calls
+    `embed_grad` by hand."""
     if dtype is None:
         out = _lib.host().embed(table, ids, ecc, scale, p, seed, offset)  # None: something to differentiate or convert first, or an error to report
         if out is not None:
@@ -123,7 +124,7 @@ def embed_grad(dy: torch.Tensor, ids: torch.Tensor, rows: int, *, scale: float =
     Row v is the sum of scale * dropout(dy) over the tokens with id v, in fp32 and in an order that depends on the ids alone (same inputs, same
     bits), rounded once; rows without a token are 0.  Into `out` where it is given (a leaf of `Zero1Optimizer.grads`, say); with `accumulate` the sums
     are added to what `out` holds (the gradient that the output head of a tied model left there, or an earlier micro-batch's), and rows without a
-    token are neither read nor written."""
+    token are neither read nor written.  `out` must not overlap dy.  Not differentiable itself."""
     if dtype is None:
         grad = _lib.host().embed_grad(dy, ids, rows, scale, p, seed, offset, out, accumulate)  # None: something to convert first, or an error to report
         if grad is not None:
@@ -191,10 +192,10 @@ class TokenGradient:
 
 def dense_gradients(params: Any, grads: Any) -> Any:
     """`grads` with every TokenGradient in it replaced by the gradient of its leaf of `params`; the same object where there is none."""
-    leaves, treedef = pytree.tree_flatten(grads)
-    if not any(isinstance(g, TokenGradient) for g in leaves):
+    if not any(type(g) is TokenGradient for g in pytree.tree_leaves(grads)):
         return grads
+    leaves, treedef = pytree.tree_flatten(grads)
     param_leaves, param_def = pytree.tree_flatten(params)
     if treedef != param_def:
         return grads  # (refused where the trees are compared)
-    return treedef.unflatten([g.dense(as_tensor(p)) if isinstance(g, TokenGradient) else g for g, p in zip(leaves, param_leaves)])
+    return treedef.unflatten([g.dense(as_tensor(p)) if type(g) is TokenGradient else g for g, p in zip(leaves, param_leaves)])

@@ -553,8 +553,8 @@ class Zero1Optimizer:
     ALL_PHASES = ("reduce_scatter", "step", "all_gather")
 
     def step(self, grads: Any = None, phases: Tuple[str, ...] = ALL_PHASES) -> Any:
-        """One optimizer step.  `grads` (optional) is copied into the flat gradient buffers;
-        leave it out when backward already wrote into `self.grads`.  Returns `self.params`.
+        """One optimizer step.  `grads` (optional) is copied into the flat gradient buffers (a TokenGradient is
+        summed up there); leave it out when backward already wrote into `self.grads`.  Returns `self.params`.
 
         `phases` is for measurement: leaving "reduce_scatter" out steps on this rank's own gradients,
         leaving "all_gather" out keeps the updated slice local (the replicas then disagree; the state
