@@ -5,7 +5,8 @@
 // atomics on values), which also says where each row's tokens begin.  (2) The sorted tokens are cut into chunks of equal length whatever their ids, so
 // that an id that half of all tokens carry costs no more than others: a warp adds up 256 columns of one chunk and writes the rows whose tokens
 // lie all in the chunk; of the row at either end that does not, it leaves a partial sum, and the warp that leaves a row's last one adds them
-// up.  (3) The rows without a token are cleared, beside (2).
+// up.  (3) The rows without a token are cleared in the launch of (2), mostly by blocks behind those of the sums.  (A launch of its own that starts beside the sums would read
+// what the sort wrote without having waited for it: only a launch's own wait makes earlier ones' writes visible to it.)
 //
 // Bound by HBM from a hundred thousand rows of some thousand columns on (32768 tokens of 4096 bf16 columns into 128256 rows: 1.32 GB in 203 us, 6.5 TB/s), by
 // latency below: the sort takes 5 to 11 us (three to six dependent trips to memory a launch), a chunk's sum as much, joining the pieces of
@@ -566,10 +567,49 @@ struct SumParams {
   unsigned long long row_bytes;  // of the gradient
   uint32_t dy_bytes;             // between rows of dY
   uint32_t rows, last_token, tiles, chunk, chunks;
+  uint32_t lead, sum_blocks, block_rows;  // rows that a warp of the sums clears, blocks of the sums, and rows that a block behind them clears
   int32_t dealt;  // starts is in the order of slot_of, not of the rows
   float factor;
   Drop drop;
 };
+
+// Which of up to 32 rows from r on have no token.
+FO_DEVI uint32_t rows_without_tokens(const SumParams& p, const uint32_t r, const uint32_t end, const int lane) {
+  const uint32_t mine = min(r + lane, end - 1), s = p.dealt ? slot_of(mine, p.rows) : mine;
+  return __ballot_sync(~0u, r + lane < end && p.starts[s] == p.starts[s + 1]);
+}
+
+constexpr int kClearThreads = kSumThreads;
+static_assert(kClearThreads == 8 * 32, "eight warps share 32 rows");
+// Rows that a block clears: long ones, one or more a warp, of about 1 / 8 of what an SM has to clear, 4 KB to `most` bytes; or a group of 32 short ones a warp.  The fewer blocks an SM
+// holds, the more a block has to do: 128256 rows of 8 KB and 66 tokens 149 us with 64 KB a block (three blocks of sum_kernel an SM), 150 with 128, 153 with 256; with dropout (two)
+// 161, 150, 152; 200000 rows of 2000 bytes 82 and 98 with 32 KB, 70 and 77 with 64, 70 and 74 with 128.
+constexpr int clear_bytes_most(const bool drop) { return drop ? 131072 : 65536; }
+static uint32_t rows_to_clear(const unsigned long long rows, const unsigned long long row_bytes, const unsigned long long most) {
+  unsigned long long bytes = rows * row_bytes / (8 * kSms);
+  bytes = bytes < 4096 ? 4096 : (bytes < most ? bytes : most);
+  return row_bytes >= kLongRow ? (uint32_t)((bytes / row_bytes + 7) / 8 * 8 + (bytes < row_bytes ? 8 : 0)) : kClearThreads;
+}
+
+// Rows that a warp of the sums with dropout clears, a few behind every four tokens, before blocks of their own clear what is left: its time goes into draws, which leave the memory idle, and
+// two such blocks leave no room on an SM for a third that clears.  16384 tokens of 768 bf16 columns into 50257 rows 34.7 us with 24 KB a warp, 38.8 with none, 36.2 with 16, 36.3 with 32 (the
+// blocks behind fill the time until the last sums are done); 8192 of 1024 into 128256 70, 75, 71, 68.  Without dropout three blocks share an SM and the sums wait for the memory: nothing gained.
+constexpr unsigned long long kLeadBytes = 24576;
+static uint32_t lead_rows(const unsigned long long rows, const unsigned long long row_bytes, const unsigned long long warps, const bool drop) {
+  if (!drop || row_bytes < kLongRow) return 0;
+  const unsigned long long share = (rows + warps - 1) / warps, most = kLeadBytes / row_bytes, lead = share < most ? share : most;
+  return (uint32_t)(lead < 32 ? lead : 32);
+}
+
+// Clears the rows without a token from r0 to r1 - 1, by a block: 32 rows at a time that the warps share where they are long, else each warp has its own.
+FO_DEVI void clear_block(const SumParams& p, const uint32_t r0, const uint32_t r1, const int lane, const int warp) {
+  const bool shared = p.row_bytes >= kLongRow;
+  for (uint32_t r = shared ? r0 : r0 + warp * 32; r < r1; r += shared ? 32 : kClearThreads) {
+    uint32_t empty = rows_without_tokens(p, r, r1, lane);
+    if (shared) empty &= 0x01010101u << warp;
+    clear_rows((char*)p.out + r * p.row_bytes, min(32u, r1 - r), empty, p.row_bytes, lane);
+  }
+}
 
 // A lane's eight columns of a row of the gradient, `to` being where they begin: neighbours, or every 32nd, so that neighbours lie in neighbouring
 // lanes (`count`: columns from the lane's first one to the end of the tile).
@@ -716,13 +756,44 @@ __global__ void __launch_bounds__(kSumThreads, sum_blocks_per_sm(DROP)) sum_kern
   extern __shared__ __align__(16) unsigned char rings[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
   const unsigned long long task = (unsigned long long)blockIdx.x * (kSumThreads / 32) + warp;
+  if constexpr (!ACC) {
+    if (blockIdx.x >= p.sum_blocks) {
+      const unsigned long long r0 = (unsigned long long)p.sum_blocks * (kSumThreads / 32) * p.lead + (unsigned long long)(blockIdx.x - p.sum_blocks) * p.block_rows;
+      if (r0 < p.rows) clear_block(p, (uint32_t)r0, (uint32_t)min(r0 + p.block_rows, (unsigned long long)p.rows), lane, warp);
+      return;
+    }
+  }
   const uint32_t tile = (uint32_t)(task % p.tiles), chunk = (uint32_t)(task / p.tiles);
-  if (chunk >= p.chunks) return;
+  // The warp's share of the first rows: which of them it has left to clear.
+  uint32_t to_clear = 0;
+  char* lead = nullptr;
+  if constexpr (DROP && !ACC) {
+    const unsigned long long r0 = task * p.lead;
+    if (p.lead != 0 && r0 < p.rows) {
+      to_clear = rows_without_tokens(p, (uint32_t)r0, (uint32_t)min(r0 + p.lead, (unsigned long long)p.rows), lane);
+      lead = (char*)p.out + r0 * p.row_bytes;
+    }
+  }
+  const auto clear_lead = [&](uint32_t most) {
+    if constexpr (DROP && !ACC) {
+      for (; to_clear != 0 && most != 0; to_clear &= to_clear - 1u, --most) {
+        char* const at = lead + (unsigned long long)(__ffs(to_clear) - 1) * p.row_bytes;
+        clear_bytes(at, at + p.row_bytes, lane);
+      }
+    }
+  };
+  if (chunk >= p.chunks) {
+    clear_lead(32);
+    return;
+  }
   const uint32_t first = (uint32_t)((unsigned long long)chunk * p.chunk);
   // keys and places of 32 tokens, one per lane; what lies behind the last token that names a row is nothing
   const uint32_t n = p.starts[p.rows];
   uint32_t key = first + lane <= p.last_token ? p.key[first + lane] : 0u, pos = first + lane <= p.last_token ? p.pos[first + lane] : 0u;
-  if (first >= n) return;
+  if (first >= n) {
+    clear_lead(32);
+    return;
+  }
   const uint32_t end = (uint32_t)min((unsigned long long)first + p.chunk, (unsigned long long)n);
   const uint32_t last_row = p.key[end - 1];
   const unsigned long long c0 = (unsigned long long)tile * kTileCols;
@@ -761,6 +832,7 @@ __global__ void __launch_bounds__(kSumThreads, sum_blocks_per_sm(DROP)) sum_kern
     if (first + k < end) fetch(k, at, k);
     copy_commit();
   }
+  const uint32_t groups = (end - first + 3) / 4, at_once = (__popc(to_clear) + groups - 1) / groups;
   float sum[8] = {};
   bool any = false;  // a row began in this chunk
   // Four tokens at a time: single ones cost a third more instructions, and with the draws of dropout in it, the loop unrolled over eight outgrew
@@ -824,6 +896,7 @@ __global__ void __launch_bounds__(kSumThreads, sum_blocks_per_sm(DROP)) sum_kern
           for (int j = 0; j < 8; ++j) sum[j] = __fmaf_rn(v[j], p.factor, sum[j]);
         }
       }
+      clear_lead(at_once);
     }
     key = next_key;
     pos = next_pos;
@@ -850,39 +923,6 @@ __global__ void __launch_bounds__(kSumThreads, sum_blocks_per_sm(DROP)) sum_kern
     const Pieces r = pieces_of(p, chunk, which == 0 ? row_begins / p.chunk : chunk, ((which == 0 ? row_ends : last_ends) - 1) / p.chunk, tile);
     if (join_pieces(p, r, tile, lane, sum)) write_row<OT, VECTORS>(out + (which == 0 ? first_row : last_row) * p.row_bytes + lane * kLaneOut, count, sum);
   }
-}
-
-// Clears the rows without a token, in blocks in the order of the rows: 7.2 TB/s, where a block per SM that walks over its share of them gets 6.2 (128256
-// rows of 8 KB).  Its blocks start beside those of the sums, which are all resident by then, so that one's waiting hides behind the other's writing.
-constexpr int kClearThreads = 256, kClearBytes = 32768;
-static_assert(kClearThreads == 8 * 32 && kSumThreads == 8 * 32, "eight warps share 32 rows");
-// Of a block: long rows, one or more a warp, of about 1 / 8 of what an SM has to clear, 4 to 32 KB; or a group of 32 short ones a warp.
-static uint32_t rows_to_clear(const unsigned long long rows, const unsigned long long row_bytes) {
-  unsigned long long bytes = rows * row_bytes / (8 * kSms);
-  bytes = bytes < 4096 ? 4096 : (bytes < kClearBytes ? bytes : kClearBytes);
-  return row_bytes >= kLongRow ? (uint32_t)((bytes / row_bytes + 7) / 8 * 8 + (bytes < row_bytes ? 8 : 0)) : kClearThreads;
-}
-
-struct ClearParams {
-  const uint32_t* starts;
-  char* out;
-  unsigned long long row_bytes;
-  uint32_t rows, per_block;
-  int32_t dealt;  // starts is in the order of slot_of, not of the rows
-};
-__global__ void __launch_bounds__(kClearThreads) clear_kernel(const __grid_constant__ ClearParams p) {
-  chain_release();  // (no wait: the sums in front have waited for the sort)
-  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-  const uint32_t r0 = blockIdx.x * p.per_block, r1 = min(r0 + p.per_block, p.rows);
-  // 32 rows at a time: the block's warps share them where they are long, else each has its own
-  const bool shared = p.row_bytes >= kLongRow;
-  for (uint32_t r = shared ? r0 : r0 + warp * 32; r < r1; r += shared ? 32 : kClearThreads) {
-    const uint32_t mine = r + lane, s = p.dealt ? slot_of(min(mine, r1 - 1), p.rows) : min(mine, r1 - 1);
-    uint32_t empty = __ballot_sync(~0u, mine < r1 && p.starts[s] == p.starts[s + 1]);
-    if (shared) empty &= 0x01010101u << warp;
-    clear_rows(p.out + r * p.row_bytes, min(32u, r1 - r), empty, p.row_bytes, lane);
-  }
-  chain_end();
 }
 
 // ---- a handful of tokens, in one launch -------------------------------------------------------------------------------
@@ -919,7 +959,7 @@ __global__ void __launch_bounds__(kSumThreads) few_kernel(const __grid_constant_
         if (key[h] >= r0 && key[h] < r1) atomicOr(&named[(key[h] - r0) / 32], 1u << ((key[h] - r0) & 31));
     }
     __syncthreads();
-    const bool shared = p.row_bytes >= kLongRow;  // (as in clear_kernel)
+    const bool shared = p.row_bytes >= kLongRow;  // (as in clear_block)
     for (uint32_t r = shared ? r0 : r0 + warp * 32; r < r1; r += shared ? 32 : kSumThreads) {
       uint32_t empty = ~named[(r - r0) / 32];
       if (shared) empty &= 0x01010101u << warp;
@@ -1009,7 +1049,7 @@ static int few_tokens(const FoEmbedGrad& f, const SumParams& s, const bool vecto
   p.token_blocks = (p.n * p.tiles + kSumThreads / 32 - 1) / (kSumThreads / 32);
   unsigned int grid = p.token_blocks;
   if (!f.accumulate) {
-    p.clear_rows = rows_to_clear(s.rows, s.row_bytes);
+    p.clear_rows = rows_to_clear(s.rows, s.row_bytes, 32768);
     grid += (p.rows + p.clear_rows - 1) / p.clear_rows;
   }
   if (grid == 0) return FO_OK;
@@ -1149,16 +1189,19 @@ extern "C" int fo_embed_grad(const FoEmbedGrad* f, void* cuda_stream) {
   X(FO_F32, FO_F32) X(FO_F32, FO_BF16) X(FO_F32, FO_F16) X(FO_BF16, FO_F32) X(FO_BF16, FO_BF16) X(FO_BF16, FO_F16) X(FO_F16, FO_F32) X(FO_F16, FO_BF16) X(FO_F16, FO_F16)
 #undef X
 #undef Y
-  const unsigned long long tasks = (unsigned long long)g.chunks * g.tiles;
+  const unsigned long long warps_per_block = kSumThreads / 32, blocks = ((unsigned long long)g.chunks * g.tiles + warps_per_block - 1) / warps_per_block;
+  p.sum_blocks = (uint32_t)blocks;
+  unsigned long long grid = blocks;
+  if (!f->accumulate) {
+    p.lead = lead_rows(p.rows, p.row_bytes, blocks * warps_per_block, p.drop.on != 0);
+    const unsigned long long led = p.lead * blocks * warps_per_block, rest = led < p.rows ? p.rows - led : 0;
+    p.block_rows = rows_to_clear(rest, p.row_bytes, clear_bytes_most(p.drop.on != 0));
+    grid += (rest + p.block_rows - 1) / p.block_rows;
+  }
   bool chained = true;
   cudaError_t e = cudaSuccess;
   // (some rings are above the 48 KB that need no leave; it is given at each call, for whichever device is current)
   if (smem > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e == cudaSuccess) e = launch_chained(kernel, (unsigned int)((tasks + kSumThreads / 32 - 1) / (kSumThreads / 32)), (unsigned int)kSumThreads, smem, chained, stream, p);
-  if (!f->accumulate && e == cudaSuccess) {
-    ClearParams c = {p.starts, (char*)f->out, p.row_bytes, p.rows, 0, p.dealt};
-    c.per_block = rows_to_clear(p.rows, p.row_bytes);
-    e = launch_chained(clear_kernel, (p.rows + c.per_block - 1) / c.per_block, (unsigned int)kClearThreads, 0, chained, stream, c);
-  }
+  if (e == cudaSuccess) e = launch_chained(kernel, (unsigned int)grid, (unsigned int)kSumThreads, smem, chained, stream, p);
   return e == cudaSuccess ? FO_OK : fail(FO_ERR_CUDA, "fo_embed_grad: launch failed: %s", cudaGetErrorString(e));
 }
