@@ -7,6 +7,7 @@ libflashoptim_b200.so on the current CUDA stream.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -29,6 +30,12 @@ def require_cuda(t: torch.Tensor, what: str) -> None:
         raise RuntimeError(
             f"{what} lives on {t.device}; flashoptim_jax_b200 computes on CUDA devices only (there is no CPU path)"
         )
+
+
+def refuse_tangent(t: torch.Tensor, what: str) -> None:
+    """A dual tensor of torch.autograd.forward_ad: the kernels would take its values and lose its tangent."""
+    if forward_ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError(f"{what} carries a forward-mode tangent; flashoptim_jax_b200 has no forward-mode derivatives")
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the handle without a Stream object around it

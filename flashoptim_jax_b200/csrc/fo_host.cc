@@ -1061,7 +1061,8 @@ bool number(PyObject* x, double& v) {
 }
 bool float_type(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
 bool int_type(at::ScalarType t) { return t == at::kInt || t == at::kLong; }
-bool differentiated(const at::Tensor& t) { return t.requires_grad() && c10::GradMode::is_enabled(); }
+// in reverse mode; or a dual tensor of forward mode, which the Python path refuses
+bool differentiated(const at::Tensor& t) { return (t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(0).defined(); }
 
 struct DropArgs {
   FoDropout f = {};
@@ -1155,7 +1156,7 @@ PyObject* embed(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
 PyObject* embed_grad(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   if (nargs != 9) { PyErr_SetString(PyExc_TypeError, "embed_grad takes 9 arguments"); return nullptr; }
   const at::Tensor* x = dense(a[0], -1);
-  if (x == nullptr || !float_type(x->scalar_type()) || x->dim() < 1 || !PyLong_CheckExact(a[2]) || !PyBool_Check(a[8])) Py_RETURN_NONE;
+  if (x == nullptr || !float_type(x->scalar_type()) || x->_fw_grad(0).defined() || x->dim() < 1 || !PyLong_CheckExact(a[2]) || !PyBool_Check(a[8])) Py_RETURN_NONE;
   const int device = x->device().index();
   const at::Tensor* i = dense(a[1], device);
   if (i == nullptr || !int_type(i->scalar_type()) || x->sizes().slice(0, x->dim() - 1) != i->sizes()) Py_RETURN_NONE;
@@ -1169,7 +1170,7 @@ PyObject* embed_grad(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   f.accumulate = a[8] == Py_True;
   if (a[7] != Py_None) {
     o = dense(a[7], device);
-    if (o == nullptr || !float_type(o->scalar_type()) || o->dim() != 2 || o->size(0) != rows || o->size(1) != dim) Py_RETURN_NONE;
+    if (o == nullptr || !float_type(o->scalar_type()) || o->_fw_grad(0).defined() || o->dim() != 2 || o->size(0) != rows || o->size(1) != dim) Py_RETURN_NONE;
   } else if (f.accumulate) {
     Py_RETURN_NONE;
   }

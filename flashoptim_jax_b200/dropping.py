@@ -14,7 +14,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._dev import DTYPE_CODE, dtype_name, require_cuda, stream_ptr
+from ._dev import DTYPE_CODE, dtype_name, refuse_tangent, require_cuda, stream_ptr
 
 
 def checked_dropout(p, seed, offset, device: torch.device) -> Tuple[float, int, int, Optional[torch.Tensor]]:
@@ -72,16 +72,18 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset=0, *, residual: Optiona
     `seed` and `offset` (whole numbers, taken modulo 2^64) and the element's place in row-major order decide what is dropped: give each layer
     a seed and each step an offset.  `offset` may be a one-element int32 or int64 CUDA tensor (the counter of a capturable
     optimizer's state, say), read when the kernel runs: a captured call then drops other elements at each replay.  Until the
-    backward pass has run it must keep its value.  Differentiable in x and residual (once); by hand, the gradient of x is
+    backward pass has run it must keep its value.  Differentiable in x and residual (once, in reverse mode); by hand, the gradient of x is
     `dropout(dy, p, seed, offset)` and that of the residual is dy."""
     y = _lib.host().dropout(x, p, seed, offset, residual)  # None: something to differentiate or convert first, or an error to report
     if y is not None:
         return y
     require_cuda(x, "x")
+    refuse_tangent(x, "x")
     if x.dtype not in DTYPE_CODE:
         raise ValueError(f"dropout takes float32, bfloat16 or float16, got {dtype_name(x.dtype)}")
     if residual is not None:
         require_cuda(residual, "residual")
+        refuse_tangent(residual, "residual")
         if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
             raise ValueError(f"residual of shape {tuple(residual.shape)}, {dtype_name(residual.dtype)}, on {residual.device} does not match "
                              f"x of shape {tuple(x.shape)}, {dtype_name(x.dtype)}, on {x.device}")

@@ -16,7 +16,7 @@ import torch
 
 from . import _lib
 from . import tree as pytree
-from ._dev import DTYPE_CODE, ECC_BITS_OF, LOW_PRECISION, as_tensor, dtype_name, require_cuda, stream_ptr
+from ._dev import DTYPE_CODE, ECC_BITS_OF, LOW_PRECISION, as_tensor, dtype_name, refuse_tangent, require_cuda, stream_ptr
 from .dropping import checked_dropout, fill_dropout
 
 _IDS_BITS = {torch.int32: 32, torch.int64: 64}
@@ -89,13 +89,14 @@ def embed(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, ecc: Op
     are the fp32 weights that `reconstruct_leaf` gives; the 0-d marker of a leaf without codes is taken for none.  The result has the table's dtype, with
     `ecc` fp32; `dtype` may ask for either.  `ids`: int32 or int64.  A negative id is no token: its row is 0 and it has no part in the
     gradient.  An id behind the last row cannot be reported without waiting for the GPU: its row is NaN, which the loss shows.
-    Differentiable in the table (once): the gradient is `embed_grad`'s, in the table's dtype.  A step that is captured in a CUDA graph calls
+    Differentiable in the table (once, in reverse mode): the gradient is `embed_grad`'s, in the table's dtype.  A step that is captured in a CUDA graph calls
     `embed_grad` by hand."""
     if dtype is None:
         out = _lib.host().embed(table, ids, ecc, scale, p, seed, offset)  # None: something to differentiate or convert first, or an error to report
         if out is not None:
             return out
     require_cuda(table, "table")
+    refuse_tangent(table, "table")
     if table.dim() != 2 or table.dtype not in DTYPE_CODE:
         raise ValueError(f"table must be a float32, bfloat16 or float16 matrix, got shape {tuple(table.shape)}, {dtype_name(table.dtype)}")
     _check_ids(ids, table.device)
@@ -130,6 +131,7 @@ def embed_grad(dy: torch.Tensor, ids: torch.Tensor, rows: int, *, scale: float =
         if grad is not None:
             return grad
     require_cuda(dy, "dy")
+    refuse_tangent(dy, "dy")
     _check_ids(ids, dy.device)
     if dy.dtype not in DTYPE_CODE:
         raise ValueError(f"dy must be float32, bfloat16 or float16, got {dtype_name(dy.dtype)}")
@@ -148,6 +150,7 @@ def embed_grad(dy: torch.Tensor, ids: torch.Tensor, rows: int, *, scale: float =
             raise ValueError(f"dtype must be float32, bfloat16 or float16, got {dtype_name(dtype)}")
     else:
         require_cuda(out, "out")
+        refuse_tangent(out, "out")
         if tuple(out.shape) != (rows, dim) or out.dtype not in DTYPE_CODE or (dtype is not None and out.dtype != dtype) or out.device != dy.device:
             raise ValueError(f"out of shape {tuple(out.shape)}, {dtype_name(out.dtype)}, on {out.device} is not a gradient of shape {(rows, dim)} on {dy.device}")
         if not out.is_contiguous():
