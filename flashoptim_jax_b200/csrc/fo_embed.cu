@@ -189,6 +189,7 @@ extern "C" int fo_embed(const FoEmbed* f, void* stream) {
   EmbedParams p;
   double factor;
   if (!make_drop(&f->dropout, p.drop, factor)) return fail(FO_ERR_INVALID_ARG, "fo_embed: p = %g (it lies in [0, 1]), dev_offset_bits = %d (32 or 64)", f->dropout.p, f->dropout.dev_offset_bits);
+  if (!make_factor(f->scale, factor, p.factor)) return fail(FO_ERR_INVALID_ARG, "fo_embed: scale %g with p = %g (scale / (1 - p) has to be 0 or a normal fp32 number)", f->scale, f->dropout.p);
   if (f->n_tokens == 0 || f->dim == 0) return FO_OK;
   if (f->ids == nullptr || f->out == nullptr || (f->rows > 0 && (f->table == nullptr || (f->ecc_bits != 0 && f->ecc == nullptr))))
     return fail(FO_ERR_INVALID_ARG, "fo_embed: null pointer");
@@ -202,7 +203,6 @@ extern "C" int fo_embed(const FoEmbed* f, void* stream) {
   p.tiles = (uint32_t)((p.dim + 255) / 256);
   p.ids_bits = f->ids_bits;
   p.out_f32 = f->out_dtype == FO_F32;
-  p.factor = (float)((double)f->scale * factor);
   const int size = size_of(f->table_dtype), code = f->ecc_bits / 8;
   const bool vectors = f->dim % 8 == 0 && on_16_bytes(f->table) && f->row_stride * size % 16 == 0 && on_16_bytes(f->out) &&
                        (code == 0 || ((uintptr_t)f->ecc % (8 * code) == 0 && f->ecc_stride % 8 == 0));

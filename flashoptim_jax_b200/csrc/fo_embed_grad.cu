@@ -1155,6 +1155,7 @@ extern "C" int fo_embed_grad(const FoEmbedGrad* f, void* cuda_stream) {
   SumParams p = {};
   double factor;
   if (!make_drop(&f->dropout, p.drop, factor)) return fail(FO_ERR_INVALID_ARG, "fo_embed_grad: p = %g (it lies in [0, 1]), dev_offset_bits = %d (32 or 64)", f->dropout.p, f->dropout.dev_offset_bits);
+  if (!make_factor(f->scale, factor, p.factor)) return fail(FO_ERR_INVALID_ARG, "fo_embed_grad: scale %g with p = %g (scale / (1 - p) has to be 0 or a normal fp32 number)", f->scale, f->dropout.p);
   if (int rc = sizes_ok("fo_embed_grad", f->rows, f->dim, f->n_tokens)) return rc;
   if (f->rows == 0 || f->dim == 0 || (f->accumulate && f->n_tokens == 0)) return FO_OK;
   if (f->out == nullptr || (f->n_tokens > 0 && (f->ids == nullptr || f->dy == nullptr))) return fail(FO_ERR_INVALID_ARG, "fo_embed_grad: null pointer");
@@ -1171,7 +1172,6 @@ extern "C" int fo_embed_grad(const FoEmbedGrad* f, void* cuda_stream) {
   p.partial = (float*)(ws + g.partial);
   p.dim = f->dim; p.dy_bytes = (uint32_t)(f->dy_stride * size_of(f->dy_dtype)); p.row_bytes = f->dim * size_of(f->out_dtype);
   p.rows = (uint32_t)f->rows; p.last_token = (uint32_t)(f->n_tokens - 1); p.dealt = !g.several; p.tiles = g.tiles; p.chunk = g.chunk; p.chunks = g.chunks;
-  p.factor = (float)(f->scale * factor);
   const bool vectors = f->dim % 8 == 0 && on_16_bytes(f->dy) && f->dy_stride * size_of(f->dy_dtype) % 16 == 0 && on_16_bytes(f->out);
   if (f->n_tokens <= kFewTokens) return few_tokens(*f, p, vectors, stream);
   if (int rc = g.several ? sort_in_memory(*f, g, stream, at) : sort_by_rows(*f, g, stream)) return rc;

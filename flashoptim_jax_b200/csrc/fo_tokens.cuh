@@ -2,6 +2,8 @@
 // fp32, and the counter-based generator behind dropout.
 #pragma once
 
+#include <cmath>
+
 #include "fo_step.cuh"
 
 namespace fo {
@@ -47,6 +49,12 @@ inline bool make_drop(const FoDropout* f, Drop& d, double& factor) {
   d.above = (uint32_t)(((uint64_t)hi + (d.lo != 0 && hi != 0xFFFFu ? 1u : 0u)) << 16) - 1u;  // (p = 1: all ones, none stays)
   factor = f->p < 1.0 ? 1.0 / (1.0 - f->p) : 0.0;
   return true;
+}
+
+// What elements that stay are multiplied by.  false: neither 0 nor a normal fp32 number (a subnormal one holds too few bits of the product)
+inline bool make_factor(const double scale, const double factor, float& out) {
+  out = (float)(scale * factor);
+  return scale * factor == 0.0 ? scale == 0.0 || factor == 0.0 : std::isnormal(out);
 }
 
 // the call's offset, part of which may lie on the device (so that a captured call drops other elements at each replay)

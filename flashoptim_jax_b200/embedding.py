@@ -87,7 +87,8 @@ def embed(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, ecc: Op
 
     `table`: (rows, dim) in float32, bfloat16 or float16.  With `ecc`, the error-correction codes of the same leaf in the optimizer state, the rows
     are the fp32 weights that `reconstruct_leaf` gives; the 0-d marker of a leaf without codes is taken for none.  The result has the table's dtype, with
-    `ecc` fp32; `dtype` may ask for either.  `ids`: int32 or int64.  A negative id is no token: its row is 0 and it has no part in the
+    `ecc` fp32; `dtype` may ask for either.  scale / (1 - p), one factor in fp32, has to be 0 or a normal
+    fp32 number.  `ids`: int32 or int64.  A negative id is no token: its row is 0 and it has no part in the
     gradient.  An id behind the last row cannot be reported without waiting for the GPU: its row is NaN, which the loss shows.
     Differentiable in the table (once, in reverse mode): the gradient is `embed_grad`'s, in the table's dtype.  A step that is captured in a CUDA graph calls
     `embed_grad` by hand."""

@@ -300,7 +300,7 @@ int fo_dropout(const void* x, const void* residual, void* y, int32_t dtype, uint
 
 /* out[t, :] = drop(scale * W[ids[t], :]), W of `rows` rows of `dim` elements, row_stride apart.  With ecc_bits 8 or 16, W is what fo_reconstruct
  * makes of (table, ecc), whose rows are ecc_stride apart.  out: n_tokens x dim without gaps, in the table's dtype or fp32; rounded once.  A negative id
- * is no token: a row of zeros.  An id behind the last row reads nothing: a row of NaN. */
+ * is no token: a row of zeros.  scale / (1 - p), which elements are multiplied by in fp32, is 0 or a normal fp32 number.  An id behind the last row reads nothing: a row of NaN. */
 typedef struct FoEmbed {
   uint32_t struct_size;
   int32_t table_dtype, out_dtype, ecc_bits, ids_bits;
