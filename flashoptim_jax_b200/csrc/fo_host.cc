@@ -1170,7 +1170,7 @@ PyObject* embed_grad(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   f.accumulate = a[8] == Py_True;
   if (a[7] != Py_None) {
     o = dense(a[7], device);
-    if (o == nullptr || !float_type(o->scalar_type()) || o->_fw_grad(0).defined() || o->dim() != 2 || o->size(0) != rows || o->size(1) != dim) Py_RETURN_NONE;
+    if (o == nullptr || !float_type(o->scalar_type()) || differentiated(*o) || o->dim() != 2 || o->size(0) != rows || o->size(1) != dim) Py_RETURN_NONE;
   } else if (f.accumulate) {
     Py_RETURN_NONE;
   }

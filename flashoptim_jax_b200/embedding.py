@@ -126,7 +126,8 @@ def embed_grad(dy: torch.Tensor, ids: torch.Tensor, rows: int, *, scale: float =
     Row v is the sum of scale * dropout(dy) over the tokens with id v, in fp32 and in an order that depends on the ids alone (same inputs, same
     bits), rounded once; rows without a token are 0.  Into `out` where it is given (a leaf of `Zero1Optimizer.grads`, say); with `accumulate` the sums
     are added to what `out` holds (the gradient that the output head of a tied model left there, or an earlier micro-batch's), and rows without a
-    token are neither read nor written.  `out` must not overlap dy.  Not differentiable itself."""
+    token are neither read nor written.  `out` must not overlap dy, nor require a gradient (but under torch.no_grad()).  Not differentiable
+    itself."""
     if dtype is None:
         grad = _lib.host().embed_grad(dy, ids, rows, scale, p, seed, offset, out, accumulate)  # None: something to convert first, or an error to report
         if grad is not None:
@@ -152,6 +153,8 @@ def embed_grad(dy: torch.Tensor, ids: torch.Tensor, rows: int, *, scale: float =
     else:
         require_cuda(out, "out")
         refuse_tangent(out, "out")
+        if out.requires_grad and torch.is_grad_enabled():  # (as torch's own operators with out=)
+            raise RuntimeError("embed_grad writes into out behind autograd's back, but out requires a gradient")
         if tuple(out.shape) != (rows, dim) or out.dtype not in DTYPE_CODE or (dtype is not None and out.dtype != dtype) or out.device != dy.device:
             raise ValueError(f"out of shape {tuple(out.shape)}, {dtype_name(out.dtype)}, on {out.device} is not a gradient of shape {(rows, dim)} on {dy.device}")
         if not out.is_contiguous():

@@ -38,3 +38,20 @@ def test_forward_mode_is_refused(name):
             call(forward_ad.make_dual(x, torch.ones_like(x)))
         call(x)  # beside dual numbers, ordinary ones are as ever
     call(x)
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_a_gradient_is_not_written_into_a_graph(accumulate):
+    """The sums know nothing of the graph that `out` belongs to: its gradient would be that of what `out` held before."""
+    import flashoptim_jax_b200 as fo
+
+    dy, ids = torch.ones(6, 8, device="cuda"), torch.arange(6, device="cuda")
+    leaf = torch.ones(9, 8, device="cuda", requires_grad=True)
+    for out in (leaf, leaf * 2):
+        before = out.detach().clone()
+        with pytest.raises(RuntimeError, match="out"):
+            fo.embed_grad(dy, ids, 9, out=out, accumulate=accumulate)
+        assert torch.equal(out.detach(), before)
+    with torch.no_grad():  # as torch's own operators with out=
+        got = fo.embed_grad(dy, ids, 9, out=leaf, accumulate=accumulate)
+    assert got is leaf and torch.equal(leaf.detach()[:6], dy + (1.0 if accumulate else 0.0))
