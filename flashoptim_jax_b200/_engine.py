@@ -22,6 +22,7 @@ import torch
 from . import _lib
 from . import tree as pytree
 from ._dev import DTYPE_CODE, ECC_BITS_OF, as_tensor, require_cuda, stream_ptr
+from .embedding import dense_leaves, has_tokens
 from .quantization import QuantizedArray
 from .utils import (
     GroupResolver,
@@ -557,7 +558,8 @@ def flush_copies() -> None:
 
 
 def flatten_step_inputs(name: str, params, grads, state_trees: List[Any]):
-    """Flatten params / grads / state trees and check that they line up (adamw.py:511-519)."""
+    """Flatten params / grads / state trees and check that they line up (adamw.py:511-519); the gradients of tables that come as
+    tokens are summed up."""
     _copies.pairs = []  # a step that failed half-way leaves nothing behind
     param_pl, treedef = _tree_leaves_with_paths(params)
     # the usual case, all trees alike, is settled by the cheap structural signatures; anything else goes
@@ -571,6 +573,8 @@ def flatten_step_inputs(name: str, params, grads, state_trees: List[Any]):
         alike = alike and sig == want and len(leaves) == len(param_pl)
         flat_states.append(leaves)
     if alike:
+        if has_tokens(grad_leaves):
+            grad_leaves = dense_leaves([p for _, p in param_pl], grad_leaves)
         return param_pl, grad_leaves, flat_states, treedef
     grad_pl, grad_def = _tree_leaves_with_paths(grads)
     for st in state_trees:
@@ -580,7 +584,7 @@ def flatten_step_inputs(name: str, params, grads, state_trees: List[Any]):
         raise ValueError(f"{name} state trees must match parameter structure")
     if [p for p, _ in param_pl] != [p for p, _ in grad_pl]:
         raise ValueError(f"{name} gradients must match parameter paths")
-    return param_pl, [g for _, g in grad_pl], flat_states, treedef
+    return param_pl, dense_leaves([p for _, p in param_pl], [g for _, g in grad_pl]), flat_states, treedef
 
 
 def make_work(

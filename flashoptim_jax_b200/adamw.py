@@ -68,7 +68,6 @@ def _make_adam_transform(learning_rate, b1, b2, eps, weight_decay, quantize, mas
         """The same step with no host scalar in it: the counter stays on the device, and the learning rate
         (a number or a 0-d CUDA tensor the caller updates), count + 1 and the bias corrections (adamw.py:510,
         526-528) are formed there by fo_step_scalars, so the call can be captured in a CUDA graph and replayed."""
-        grads = dense_gradients(params, grads)
         param_pl, grad_leaves, (ecc_leaves, mu_leaves, nu_leaves), treedef = eng.flatten_step_inputs(
             name, params, grads, [state.ecc, state.mu, state.nu])
         leaves = [as_tensor(leaf) for _, leaf in param_pl]
@@ -89,7 +88,7 @@ def _make_adam_transform(learning_rate, b1, b2, eps, weight_decay, quantize, mas
 
     def step_fn(params: Any, state: FlashAdamState, grads: Any):
         hit = native.run(params, state.count, (state.ecc, state.mu, state.nu), grads)
-        if hit is None and (dense := dense_gradients(params, grads)) is not grads:
+        if hit is None and native.plans and (dense := dense_gradients(params, grads)) is not grads:
             grads = dense
             hit = native.run(params, state.count, (state.ecc, state.mu, state.nu), grads)
         if hit is not None:

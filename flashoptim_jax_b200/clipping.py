@@ -19,7 +19,7 @@ from . import _engine as eng
 from . import _lib
 from . import tree as pytree
 from ._dev import as_tensor
-from .embedding import dense_gradients
+from .embedding import dense_gradients, has_tokens
 from .utils import FlashOptimizer
 
 
@@ -40,8 +40,15 @@ def clip_by_global_norm(tx: FlashOptimizer, max_norm: float) -> FlashOptimizer:
     def step_fn(params: Any, state: Any, grads: Any):
         sq = _lib.host().sq_norm(grads)
         if sq is None:
-            grads = dense_gradients(params, grads)
-            sq = global_sq_norm(grads)
+            leaves = pytree.tree_leaves(grads)
+            if has_tokens(leaves):
+                dense = dense_gradients(params, grads)
+                if dense is grads:
+                    raise ValueError("gradients must match parameter structure")
+                grads = dense
+                sq = global_sq_norm(grads)
+            else:
+                sq = eng.sq_norm_of([as_tensor(g) for g in leaves])
         with eng.grad_clip(sq, max_norm):
             params, opt_state = tx.step(params, state["opt"], grads)
         return params, {"clip": (), "opt": opt_state}

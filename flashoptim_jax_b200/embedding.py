@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from typing import Any, Optional, Tuple
+from typing import Any, List, Optional, Tuple
 
 import torch
 
@@ -197,12 +197,23 @@ class TokenGradient:
         return embed_grad(self.dy, self.ids, param.shape[0], scale=self.scale, p=self.p, seed=self.seed, offset=self.offset, out=out)
 
 
+def has_tokens(leaves: List[Any]) -> bool:
+    return any(type(g) is TokenGradient for g in leaves)
+
+
+def dense_leaves(params: List[Any], grads: List[Any]) -> List[Any]:
+    """Leaves of gradients with every TokenGradient replaced by the gradient of its parameter; the same list where there is none."""
+    if not has_tokens(grads):
+        return grads
+    return [g.dense(as_tensor(p)) if type(g) is TokenGradient else g for g, p in zip(grads, params)]
+
+
 def dense_gradients(params: Any, grads: Any) -> Any:
     """`grads` with every TokenGradient in it replaced by the gradient of its leaf of `params`; the same object where there is none."""
-    if not any(type(g) is TokenGradient for g in pytree.tree_leaves(grads)):
+    if not has_tokens(pytree.tree_leaves(grads)):
         return grads
     leaves, treedef = pytree.tree_flatten(grads)
     param_leaves, param_def = pytree.tree_flatten(params)
     if treedef != param_def:
         return grads  # (refused where the trees are compared)
-    return treedef.unflatten([g.dense(as_tensor(p)) if type(g) is TokenGradient else g for g, p in zip(leaves, param_leaves)])
+    return treedef.unflatten(dense_leaves(param_leaves, leaves))

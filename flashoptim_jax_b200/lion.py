@@ -56,7 +56,6 @@ def flash_lion(learning_rate=1e-4, b1: float = 0.9, b2: float = 0.99, weight_dec
     def capturable_step_fn(params: Any, state: FlashLionState, grads: Any):
         """The same step with no host scalar in it (counter and learning rate stay on the device, see
         flash_adamw(capturable=True)): capturable in a CUDA graph."""
-        grads = dense_gradients(params, grads)
         param_pl, grad_leaves, (ecc_leaves, mu_leaves), treedef = eng.flatten_step_inputs(
             name, params, grads, [state.ecc, state.mu])
         leaves = [as_tensor(leaf) for _, leaf in param_pl]
@@ -74,7 +73,7 @@ def flash_lion(learning_rate=1e-4, b1: float = 0.9, b2: float = 0.99, weight_dec
 
     def step_fn(params: Any, state: FlashLionState, grads: Any):
         hit = native.run(params, state.count, (state.ecc, state.mu), grads)
-        if hit is None and (dense := dense_gradients(params, grads)) is not grads:
+        if hit is None and native.plans and (dense := dense_gradients(params, grads)) is not grads:
             grads = dense
             hit = native.run(params, state.count, (state.ecc, state.mu), grads)
         if hit is not None:

@@ -70,7 +70,6 @@ def _make_sgd_transform(learning_rate, momentum, dampening, weight_decay, nester
     def capturable_step_fn(params: Any, state: FlashSGDState, grads: Any):
         """The same step with no host scalar in it (counter and learning rate stay on the device, see
         flash_adamw(capturable=True)): capturable in a CUDA graph."""
-        grads = dense_gradients(params, grads)
         param_pl, grad_leaves, (ecc_leaves, mu_leaves), treedef = eng.flatten_step_inputs(
             name, params, grads, [state.ecc, state.mu])
         leaves = [as_tensor(leaf) for _, leaf in param_pl]
@@ -93,7 +92,7 @@ def _make_sgd_transform(learning_rate, momentum, dampening, weight_decay, nester
 
     def step_fn(params: Any, state: FlashSGDState, grads: Any):
         hit = native.run(params, state.count, (state.ecc, state.mu), grads)
-        if hit is None and (dense := dense_gradients(params, grads)) is not grads:
+        if hit is None and native.plans and (dense := dense_gradients(params, grads)) is not grads:
             grads = dense
             hit = native.run(params, state.count, (state.ecc, state.mu), grads)
         if hit is not None:
