@@ -23,8 +23,8 @@ FO_DEVI float dropped(const float x, const float r, const bool keep, const float
   return RES ? fadd(r, v) : v;
 }
 
-// Bound by HBM: n elements read (twice with a residual) and written, 16 bytes at a time.  67 M bf16 elements 45 us (6.0 TB/s; 40 with p = 0, without the draws),
-// with a residual 58 (6.9 TB/s), 16 M fp32 elements 18 (7.1).  A draw keeps the multiply pipe busy for 80 cycles a warp: drawn before the loaded
+// Bound by HBM: n elements read (twice with a residual) and written, 16 bytes at a time.  Calls in a graph, where part of a result stays in the L2 until the next call: 67 M bf16 elements
+// 45 us (40 with p = 0, without the draws), with a residual 58, 16 M fp32 elements 18 to 19; as calls of their own 65 (6.2 TB/s) and 20.8 (6.1).  A draw keeps the multiply pipe busy for 80 cycles a warp: drawn before the loaded
 // elements are touched, it hides behind them (drawn after: 59, 78 and 22 us).  A launch of as many blocks as there is work, two blocks of eight elements a
 // thread: with one 67 us without a residual and p = 0, with four as long and more registers.
 template <int DT, bool RES>

@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(kEmbedThreads) embed_kernel(const __grid_const
 
 // Any width, stride and alignment: a warp per 256 columns of a token, every 32nd of them to a lane, so that neighbours lie in neighbouring lanes.  The id and
 // all addresses are the warp's, worked out once; each lane draws for eight neighbours and hands them on.  5003 tokens of 1777 columns, fp16 with 16-bit codes, to
-// fp32: 12.4 us (57 MB); eight neighbouring results per thread, whatever rows they lie in, took 27.
+// fp32: 12.8 us in a graph (57 MB); eight neighbouring results per thread, whatever rows they lie in, took 27.
 template <int DT, int ECC, bool F32>
 __global__ void __launch_bounds__(kEmbedThreads) embed_any_kernel(const __grid_constant__ EmbedParams p) {
   chain_wait();

@@ -8,10 +8,10 @@
 // up.  (3) The rows without a token are cleared in the launch of (2), mostly by blocks behind those of the sums.  (A launch of its own that starts beside the sums would read
 // what the sort wrote without having waited for it: only a launch's own wait makes earlier ones' writes visible to it.)
 //
-// Bound by HBM from a hundred thousand rows of some thousand columns on (32768 tokens of 4096 bf16 columns into 128256 rows: 1.32 GB in 203 us, 6.5 TB/s), by
+// Bound by HBM from a hundred thousand rows of some thousand columns on (32768 tokens of 4096 bf16 columns into 128256 rows: 1.32 GB in 204 us, 6.5 TB/s), by
 // latency below: the sort takes 5 to 11 us (three to six dependent trips to memory a launch), a chunk's sum as much, joining the pieces of
-// frequent rows 3 to 5.  16384 tokens of 768 columns into 50257 rows, 102 MB: 30 us, 34 with dropout; 8192 tokens of 4096 columns added to what 128256
-// rows hold: 39; 33 tokens: 7.6.
+// frequent rows 3 to 5.  16384 tokens of 768 columns into 50257 rows, 102 MB: 31 us, 35 with dropout; 8192 tokens of 4096 columns added to what 128256
+// rows hold: 39; 33 tokens: 7.5.  (Times in this file: whole calls in a graph, three sets of inputs in turn.)
 #include "fo_tokens.cuh"
 
 namespace fo {
@@ -21,24 +21,26 @@ constexpr int kSms = 148;
 // ---- sizes and the workspace ----------------------------------------------------------------------------------------
 constexpr int kTileCols = 256;     // columns of a warp: eight per lane
 constexpr int kSumThreads = 256;
-// Resident blocks per SM, and as many warps wanted, all of them resident at once.  With dropout the registers of a third block are worth more to the draws (60000 tokens
-// of 1024 columns 80 us, 86 with three; without it 59 and 56).
+// Resident blocks per SM; about as many warps are wanted as are resident.  With dropout the registers of a third block are worth more to the draws (60000 tokens
+// of 1024 columns into 50257 rows 80 us, 89 with three; without it 61 with two and 59 with three).
 constexpr int sum_blocks_per_sm(const bool drop) { return drop ? 2 : 3; }
 constexpr int kLeastChunk = 2;     // tokens
 constexpr uint32_t kFewTokens = 64;  // up to so many take one launch and no workspace
 
-// The sort by rows: 128 blocks, a 16-bit counter per row and warp; in one launch up to kSortAlone tokens (8191 tokens, 2999 rows, whole calls: 34 us, 38 in two
-// launches; 8192 and 128256: 39.8 and 38.7; 16384 and 50257: 40.2 and 37.6), else in two.
+// The sort by rows: 128 blocks, a 16-bit counter per row and warp; in one launch up to kSortAlone tokens, else in two, whatever
+// the rows: the two ways meet near 8192 tokens (4096 tokens into 2999 rows 19.8 us in one launch and 23.0 in two, 2048 added to 128256 15.6 and 17.9; 8191 into 2999 29.3 and 29.6, 8192 into 50257
+// 28.5 and 28.4, added to 128256 38.8 and 37.6, to 262143 20.0 and 20.6; 16384 into 50257 36.3 and 31.3).
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kSortRows = 2048;                      // of a block, at most
 constexpr uint32_t kSortBlocks = 128;
 constexpr unsigned long long kSortMost = 65536;      // tokens
 constexpr unsigned long long kSortAlone = 8192;  // of which up to so many take one launch
 constexpr int kSortSmem = 220 * 1024;
-static_assert(kSortRows == 2 * kSortThreads && (kSortWarps * 2 + 4) * (kSortRows + 2) <= kSortSmem && kSortMost <= 65536, "two rows a thread, shared memory, places that fit the counters");
+static_assert(kSortRows == 2 * kSortThreads && (kSortWarps * 2 + 4) * (kSortRows + 2) + 4 * kSortAlone <= kSortSmem && kSortMost <= 65536 && kSortAlone % kSortThreads == 0,
+              "two rows a thread, counters and lists in shared memory, places that fit the counters");
 // More than 65536 tokens (a place no longer fits 16 bits) or 262143 rows (nor do the counters the shared memory): the sort by digits, three launches for each
-// digit of at most nine bits, tiles of 4096 tokens.  It takes as long whatever the ids are: 131072 tokens of 768 columns into 50257 rows 89 us, where the sort by rows with counters
-// of 32 bits took 76, but 130 with 0.4 of the tokens of one id, which are all one block's.
+// digit of at most nine bits, tiles of 4096 tokens.  It takes as long whatever the ids are: 131072 tokens of 768 columns into 50257 rows 97 us, 96 with 0.4 of the tokens of one id, where
+// a sort by rows with counters of 32 bits took 13 less, and 41 more with that id, whose tokens are all one block's.
 constexpr int kDigitMax = 9, kBinsMax = 1 << kDigitMax;
 constexpr int kRadixThreads = 512, kRadixRounds = 8, kRadixTile = kRadixThreads * kRadixRounds;
 
@@ -59,7 +61,7 @@ static GradPlan plan_of(const unsigned long long rows, const unsigned long long 
   }
   g.several = n > kSortMost || rows >= (unsigned long long)kSortBlocks * kSortRows;
   const unsigned long long width = (rows / kSortBlocks + 2) & ~1ull, lists = 4 * ((n + kSortThreads - 1) / kSortThreads * kSortThreads);
-  g.alone = !g.several && n <= kSortAlone && (kSortWarps * 2 + 4) * width + lists <= kSortSmem;
+  g.alone = !g.several && n <= kSortAlone;
   g.sort_smem = g.several ? 0u : (unsigned int)((kSortWarps * 2 + 4) * width + (g.alone ? lists : 0));
   g.tiles = (uint32_t)((dim + kTileCols - 1) / kTileCols);
   const unsigned long long warps = kSms * sum_blocks_per_sm(drop) * kSumThreads / 32;
@@ -271,7 +273,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const __grid_constan
 
 // More tokens than kSortAlone: two launches.  In the first, each block deals its 2048 tokens out to 128 piles by id % 128, each pile in the order of the
 // tokens; in the second, block b takes the b-th piles of all, block after block, and puts their tokens in the order of the rows.  The work does not grow
-// with blocks x tokens as above, where 32768 tokens took 29 us.  Bound by latency: about 11 us for 16384 tokens, beside one another, of which the loads and the
+// with blocks x tokens as above, where the sort of 32768 tokens took 29 us.  Bound by latency: about 11 us for 16384 tokens, beside one another, of which the loads and the
 // barriers between them are most.
 constexpr int kDealTokens = 2 * kSortThreads;
 constexpr uint32_t kDealBlocksMost = kSortMost / kDealTokens;
@@ -928,7 +930,7 @@ __global__ void __launch_bounds__(kSumThreads, sum_blocks_per_sm(DROP)) sum_kern
 // ---- a handful of tokens, in one launch -------------------------------------------------------------------------------
 // Every block reads all ids.  A warp per token and 256 columns sees whether its token is the first with its id, and then adds up the rows of all that
 // have it, in their order; the blocks behind clear the rows that none names.  Bound by launching and by the latency of ids and rows, which the three
-// launches above pay several times (33 tokens of 1024 fp32 columns into 8192 rows, 33.6 MB: 7.6 us, 11.5 through them).  A row of k tokens takes k / 4 trips
+// launches above pay several times (64 tokens of 1024 fp32 columns into 8192 rows, 33.6 MB: 7.6 us; 65 through them 12.3).  A row of k tokens takes k / 4 trips
 // to memory, so it ends at 64.
 struct FewParams {
   const void* dy;

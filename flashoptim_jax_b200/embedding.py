@@ -123,10 +123,10 @@ def embed_grad(dy: torch.Tensor, ids: torch.Tensor, rows: int, *, scale: float =
                dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None, accumulate: bool = False) -> torch.Tensor:
     """Gradient of `embed(table, ids, ...)` for a table of `rows` rows, given that of its result: (rows, dim), in dy's dtype or `dtype`.
 
-    Row v is the sum of scale * dropout(dy) over the tokens with id v, in fp32 and in an order that depends on the ids alone (same inputs, same
-    bits), rounded once; rows without a token are 0.  Into `out` where it is given (a leaf of `Zero1Optimizer.grads`, say); with `accumulate` the sums
-    are added to what `out` holds (the gradient that the output head of a tied model left there, or an earlier micro-batch's), and rows without a
-    token are neither read nor written.  `out` must not overlap dy, nor require a gradient (but under torch.no_grad()).  Not differentiable
+    Row v is the sum of scale * dropout(dy) over the tokens with id v, in fp32 and in an order fixed by the ids, the sizes, `accumulate` and whether there is
+    dropout (same inputs, same bits), rounded once; rows without a token are 0.  Into `out` where it is given (a leaf of `Zero1Optimizer.grads`, say); with `accumulate` the sums
+    go on from what `out` holds (the gradient that the output head of a tied model left there, or an earlier micro-batch's), and rows without a
+    token are not written.  `out` must not overlap dy, nor require a gradient (but under torch.no_grad()).  Not differentiable
     itself."""
     if dtype is None:
         grad = _lib.host().embed_grad(dy, ids, rows, scale, p, seed, offset, out, accumulate)  # None: something to convert first, or an error to report

@@ -316,8 +316,8 @@ typedef struct FoEmbed {
 int fo_embed(const FoEmbed* desc, void* cuda_stream);
 
 /* The gradient of fo_embed: out[v, :] = sum over the tokens t with ids[t] = v of drop'(scale * dy[t, :]), in fp32, in an order that depends on
- * the ids alone (same inputs, same bits), rounded once; rows without a token are cleared.  accumulate != 0: the sum is added to
- * out[v, :] in fp32 before that rounding, and rows without a token are left alone.  out: rows x dim without gaps; dy: n_tokens rows, dy_stride apart.
+ * the ids, the sizes, accumulate and whether there is dropout (same inputs, same bits), rounded once; rows without a token are cleared.  accumulate != 0: out[v, :] is one
+ * term of its sum, the first or the last, and rows without a token are not written.  out: rows x dim without gaps; dy: n_tokens rows, dy_stride apart.
  * Ids that name no row are left out.  workspace: fo_embed_grad_workspace bytes of device memory, aligned to 16, which calls on one stream
  * may share.  Fewer than 2^31 - 1 tokens and rows, dim below 2^24. */
 typedef struct FoEmbedGrad {
