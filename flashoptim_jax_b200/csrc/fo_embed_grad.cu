@@ -10,7 +10,7 @@
 //
 // Bound by HBM from a hundred thousand rows of some thousand columns on (32768 tokens of 4096 bf16 columns into 128256 rows: 1.32 GB in 204 us, 6.5 TB/s), by
 // latency below: the sort takes 5 to 11 us (three to six dependent trips to memory a launch), a chunk's sum as much, joining the pieces of
-// frequent rows 3 to 5.  16384 tokens of 768 columns into 50257 rows, 102 MB: 31 us, 35 with dropout; 8192 tokens of 4096 columns added to what 128256
+// frequent rows 3 to 5.  16384 tokens of 768 columns into 50257 rows, 102 MB: 31 us, 34 with dropout; 8192 tokens of 4096 columns added to what 128256
 // rows hold: 39; 33 tokens: 7.5.  (Times in this file: whole calls in a graph, three sets of inputs in turn.)
 #include "fo_tokens.cuh"
 
@@ -594,8 +594,8 @@ static uint32_t rows_to_clear(const unsigned long long rows, const unsigned long
 }
 
 // Rows that a warp of the sums with dropout clears, a few behind every four tokens, before blocks of their own clear what is left: its time goes into draws, which leave the memory idle, and
-// two such blocks leave no room on an SM for a third that clears.  16384 tokens of 768 bf16 columns into 50257 rows 34.7 us with 24 KB a warp, 38.8 with none, 36.2 with 16, 36.3 with 32 (the
-// blocks behind fill the time until the last sums are done); 8192 of 1024 into 128256 70, 75, 71, 68.  Without dropout three blocks share an SM and the sums wait for the memory: nothing gained.
+// two such blocks leave no room on an SM for a third that clears.  16384 tokens of 768 bf16 columns into 50257 rows 34.4 us with 24 KB a warp, 38.8 with none, 35.9 with 16, 35.4 with 32 (the
+// blocks behind fill the time until the last sums are done); 60000 67.0, 70.9, 66.6, 70.2.  Without dropout three blocks share an SM and the sums wait for the memory: nothing gained.
 constexpr unsigned long long kLeadBytes = 24576;
 static uint32_t lead_rows(const unsigned long long rows, const unsigned long long row_bytes, const unsigned long long warps, const bool drop) {
   if (!drop || row_bytes < kLongRow) return 0;
@@ -766,15 +766,17 @@ __global__ void __launch_bounds__(kSumThreads, sum_blocks_per_sm(DROP)) sum_kern
     }
   }
   const uint32_t tile = (uint32_t)(task % p.tiles), chunk = (uint32_t)(task / p.tiles);
-  // The warp's share of the first rows: which of them it has left to clear.
-  uint32_t to_clear = 0;
+  // The warp's share of the first rows, a lane's where its tokens begin and end: asked for here, looked at when the first tokens are on their way.
+  uint32_t lead_begins = 0, lead_ends = 1, to_clear = 0;
   char* lead = nullptr;
   if constexpr (DROP && !ACC) {
-    const unsigned long long r0 = task * p.lead;
-    if (p.lead != 0 && r0 < p.rows) {
-      to_clear = rows_without_tokens(p, (uint32_t)r0, (uint32_t)min(r0 + p.lead, (unsigned long long)p.rows), lane);
-      lead = (char*)p.out + r0 * p.row_bytes;
+    const unsigned long long r0 = task * p.lead, r = r0 + lane;
+    if ((uint32_t)lane < p.lead && r < p.rows) {
+      const uint32_t s = p.dealt ? slot_of((uint32_t)r, p.rows) : (uint32_t)r;
+      lead_begins = p.starts[s];
+      lead_ends = p.starts[s + 1];
     }
+    lead = (char*)p.out + r0 * p.row_bytes;
   }
   const auto clear_lead = [&](uint32_t most) {
     if constexpr (DROP && !ACC) {
@@ -784,8 +786,12 @@ __global__ void __launch_bounds__(kSumThreads, sum_blocks_per_sm(DROP)) sum_kern
       }
     }
   };
-  if (chunk >= p.chunks) {
+  const auto clear_all = [&]() {
+    if constexpr (DROP && !ACC) to_clear = __ballot_sync(~0u, lead_begins == lead_ends);
     clear_lead(32);
+  };
+  if (chunk >= p.chunks) {
+    clear_all();
     return;
   }
   const uint32_t first = (uint32_t)((unsigned long long)chunk * p.chunk);
@@ -793,7 +799,7 @@ __global__ void __launch_bounds__(kSumThreads, sum_blocks_per_sm(DROP)) sum_kern
   const uint32_t n = p.starts[p.rows];
   uint32_t key = first + lane <= p.last_token ? p.key[first + lane] : 0u, pos = first + lane <= p.last_token ? p.pos[first + lane] : 0u;
   if (first >= n) {
-    clear_lead(32);
+    clear_all();
     return;
   }
   const uint32_t end = (uint32_t)min((unsigned long long)first + p.chunk, (unsigned long long)n);
@@ -834,6 +840,7 @@ __global__ void __launch_bounds__(kSumThreads, sum_blocks_per_sm(DROP)) sum_kern
     if (first + k < end) fetch(k, at, k);
     copy_commit();
   }
+  if constexpr (DROP && !ACC) to_clear = __ballot_sync(~0u, lead_begins == lead_ends);
   const uint32_t groups = (end - first + 3) / 4, at_once = (__popc(to_clear) + groups - 1) / groups;
   float sum[8] = {};
   bool any = false;  // a row began in this chunk
