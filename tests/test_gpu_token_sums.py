@@ -134,3 +134,20 @@ def test_a_captured_step_on_token_gradients():
         graph.replay()
         for x, y in zip(pytree.tree_leaves((p2, s2)), eager[k]):
             assert torch.equal(x, y), k
+
+
+@pytest.mark.parametrize("p", [0.0, 0.5])
+@pytest.mark.parametrize("n", [64, 65, 9000])
+def test_rows_are_cleared_behind_the_reach_of_32_bits(n, p):
+    """A gradient of 2.2e9 elements, 4.4 GB: every row without a token is cleared, every other one written, wherever it lies."""
+    import flashoptim_jax_b200 as fo
+
+    rows, dim = 540_000, 4104
+    ids = torch.linspace(0, rows - 1, n, dtype=torch.float64).round().long().cuda()
+    dy = (whole((n, 1), n) + 20.0).expand(n, dim).bfloat16()  # no zeros
+    out = torch.full((rows, dim), 9.0, dtype=torch.bfloat16, device="cuda")
+    fo.embed_grad(dy, ids, rows, p=p, seed=1, out=out)
+    want = fo.dropout(dy, p, 1)
+    assert torch.equal(out[ids], want)
+    out[ids] = 0
+    assert not out.any()
