@@ -319,7 +319,7 @@ int fo_embed(const FoEmbed* desc, void* cuda_stream);
  * the ids, the sizes, accumulate and whether there is dropout (same inputs, same bits), rounded once; rows without a token are cleared.  accumulate != 0: out[v, :] is one
  * term of its sum, the first or the last, and rows without a token are not written.  out: rows x dim without gaps; dy: n_tokens rows, dy_stride apart.
  * Ids that name no row are left out.  workspace: fo_embed_grad_workspace bytes of device memory, aligned to 16, which calls on one stream
- * may share.  Fewer than 2^31 - 1 tokens and rows, dim below 2^24. */
+ * may share.  Nothing else may write ids or dy while the call's launches run: ids are read more than once.  Fewer than 2^31 - 1 tokens and rows, dim below 2^24. */
 typedef struct FoEmbedGrad {
   uint32_t struct_size;
   int32_t dy_dtype, out_dtype, ids_bits, accumulate;
